@@ -73,6 +73,7 @@ const char* svdq_version(void);
  * Codes: 0x101-0x303 GEMM waits (0x302: a split tile's owner waited for a
  * partial), 0x41xx activation-pass waits, 0x4200 an
  * activation group scale above 65504/7 (the fp16 GEMM operand a16 overflowed),
+ * 0x501-0x6FF waits of the block-scaled GEMMs,
  * 0x7E01 the diagnostic wait below; the first failure since the last clear is kept.
  */
 int svdq_device_error(int* code, int clear);
@@ -451,6 +452,70 @@ int svdq_packed_gemm_plan(int M, int N, int K_pad, int* out4);
  */
 int svdq_quantize_weight(const float* w, int64_t ldw, int N, int K, int group,
                          void* out_packed, void* out_scales, int scale_dtype, cudaStream_t stream);
+
+/*
+ * Block-scaled (microscaled) floating point.  A matrix [rows, K] is held as codes and one scale per
+ * block of neighbouring columns of a row:
+ *   SVDQ_MX_NVFP4  e2m1 codes (4 bits), blocks of 16, e4m3 scales, one fp32 scale per tensor:
+ *                  scale = e4m3(amax / (6 g)), code = e2m1(x / (scale g)), value = code * scale * g
+ *   SVDQ_MX_MXFP4  e2m1 codes, blocks of 32, e8m0 scales: scale = 2^(floor(log2 amax) - 2)
+ *   SVDQ_MX_MXFP8  e4m3 codes (8 bits), blocks of 32, e8m0 scales: scale = 2^(floor(log2 amax) - 8)
+ * All roundings are to nearest, ties to even, of the exact quotient, and saturate at the largest code
+ * (6, 448) or scale (448, 2^127).  A block with an infinity or a NaN has a NaN scale (0x7F or 0xFF)
+ * and zero codes, and reads back as NaN.
+ *   codes   [rows, K_pad] columns, K_pad = round_up(K, 128), zero past K; 4-bit codes two to a byte,
+ *           the even column in the low half
+ *   scales  bytes in 512-byte tiles of 128 rows x 4 blocks: byte (row % 32) * 16 + (row / 32 % 4) * 4
+ *           + block % 4 of tile (row / 128) * (K_pad / block size / 4) + block / 4; zero past the last row.
+ *           svdq_mx_scale_bytes() bytes.
+ * The reference keeps INT4 only; these are the formats that the tensor cores scale in hardware.
+ */
+enum svdq_mx_format { SVDQ_MX_NVFP4 = 0, SVDQ_MX_MXFP4 = 1, SVDQ_MX_MXFP8 = 2 };
+
+/* Bytes of the scales of a [rows, K] matrix (0 for sizes or formats that do not exist). */
+size_t svdq_mx_scale_bytes(int rows, int K, int format);
+
+/*
+ * Quantises x [M, K] (dtype, row stride ldx elements, any alignment of its elements) as above.
+ * tensor_scale: one fp32 value on the device (nvfp4 only; NULL for 1).  codes and scales 16-byte
+ * aligned; both are written in full.  M * K_pad < 2^35 (rows counted to a multiple of 128).
+ */
+int svdq_mx_quantize(const void* x, int64_t ldx, int dtype, int M, int K, int format,
+                     const float* tensor_scale, void* codes, void* scales, cudaStream_t stream);
+
+/* Reads codes and scales back as out [M, K] (dtype, row stride ldo): code * (scale * g) in fp32,
+ * rounded once to dtype. */
+int svdq_mx_dequantize(const void* codes, const void* scales, int format, const float* tensor_scale,
+                       int M, int K, void* out, int64_t ldo, int dtype, cudaStream_t stream);
+
+/* *out = max |x| / (6 * 448), the nvfp4 tensor scale that puts the largest element on the largest
+ * code and scale; 1 for a matrix of zeros, NaN where x has a NaN. */
+int svdq_mx_tensor_scale(const void* x, int64_t ldx, int dtype, int M, int K, float* out, cudaStream_t stream);
+
+/*
+ * Block-scaled GEMM: out[m, n] = g_a g_w sum_k A[m, k] W[n, k] + bias[n], on the tensor cores'
+ * block-scaled MMAs with fp32 accumulation.  Formats (activations x weight): nvfp4 x nvfp4,
+ * mxfp4 x mxfp4, mxfp8 x mxfp4.  Tensor scales: one fp32 device value each (nvfp4 only; NULL for 1).
+ * bias [N] bf16 or NULL.  out [M, N] in out_dtype, row stride ldo >= N, any N.  The sums are added in
+ * a fixed order: the same call gives the same bits.
+ *   codes and scales 32-byte aligned; M, N <= 2^24, K <= 2^28.
+ */
+int svdq_mx_gemm(const void* a_codes, const void* a_scales, int a_format, const float* a_tensor_scale,
+                 const void* w_codes, const void* w_scales, int w_format, const float* w_tensor_scale,
+                 const void* bias, void* out, int out_dtype, int64_t ldo, int M, int N, int K,
+                 cudaStream_t stream);
+
+/*
+ * Root-mean-square norm with the residual's addition, written as mxfp8:
+ *   h = x + residual (rounded to dtype; stored to sum),  y = h * rsqrt(mean(h^2) + eps) * weight,
+ *   y quantised to SVDQ_MX_MXFP8 from fp32.
+ * x, residual, sum [M, H] and weight [H] in dtype (bf16, fp16, fp32), row strides ldx, ldr, lds;
+ * residual and sum both NULL: h = x.  weight NULL: ones.  sum may be x or residual itself (with the
+ * same stride).  codes [M, round_up(H, 128)] and scales as svdq_mx_quantize writes them.
+ */
+int svdq_rms_norm_mx(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight,
+                     int dtype, float eps, int M, int H, void* codes, void* scales, void* sum, int64_t lds,
+                     cudaStream_t stream);
 
 /*
  * Block-weight prefetcher.  Replaces the synchronous per-tensor `.to(device)`

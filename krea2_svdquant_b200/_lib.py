@@ -81,9 +81,20 @@ SIGNATURES = {
     "svdq_packed_gemm_plan": ([c_int, c_int, c_int, ctypes.POINTER(c_int)], c_int),
     "svdq_w4a4_gemm_narrow": ([c_void_p, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
                                c_int, c_void_p, c_void_p, c_int, c_int64, c_int, c_int, c_int, c_void_p], c_int),
+    "svdq_mx_scale_bytes": ([c_int, c_int, c_int], ctypes.c_size_t),
+    "svdq_mx_quantize": ([c_void_p, c_int64, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p],
+                         c_int),
+    "svdq_mx_dequantize": ([c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_void_p, c_int64, c_int, c_void_p],
+                           c_int),
+    "svdq_mx_tensor_scale": ([c_void_p, c_int64, c_int, c_int, c_int, c_void_p, c_void_p], c_int),
+    "svdq_mx_gemm": ([c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
+                      c_int, c_int64, c_int, c_int, c_int, c_void_p], c_int),
+    "svdq_rms_norm_mx": ([c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, ctypes.c_float, c_int, c_int,
+                          c_void_p, c_void_p, c_void_p, c_int64, c_void_p], c_int),
 }
 
 SVDQ_BF16, SVDQ_FP16, SVDQ_FP32 = 0, 1, 2
+SVDQ_MX_NVFP4, SVDQ_MX_MXFP4, SVDQ_MX_MXFP8 = 0, 1, 2
 SVDQ_EPI_NONE, SVDQ_EPI_ADD, SVDQ_EPI_SIGMOID_MUL, SVDQ_EPI_SILU_MUL = 0, 1, 2, 3
 STATUS_NAMES = {0: "SVDQ_OK", 1: "SVDQ_ERR_INVALID_ARGUMENT", 2: "SVDQ_ERR_UNSUPPORTED",
                 3: "SVDQ_ERR_CUDA", 4: "SVDQ_ERR_TIMEOUT", 5: "SVDQ_ERR_DEVICE_WAIT"}

@@ -1,0 +1,315 @@
+// Block-scaled GEMM for one CTA per tile, with the weight's rows as the MMA's M and the tokens as its
+// N, and K split over a cluster:  out[m, n] = alpha * sum_k A[m, k] W[n, k] + bias[n].
+//
+// With few tokens the product is bound by the weight's bytes (0.56 per element with nvfp4).  The
+// codes need no conversion on the way: TMA brings them to shared memory and the MMA reads them
+// there, with the scales in tensor memory.  A CTA streams 128 weight rows against up to 128 tokens;
+// where the tiles leave SMs idle, the CTAs of a cluster take a share of K each and add their fp32
+// partial tiles through distributed shared memory in rank order (the same result every time).
+// 6 warps: 0-3 epilogue, 4 TMA producer, 5 MMA and scale copies.
+#include "mx_gemm.cuh"
+
+namespace svdq {
+
+int make_code_map(CUtensorMap* map, const void* codes, int fmt, bool spread, int rows, int k_pad, int box_rows) {
+  const uint64_t row_bytes = (uint64_t)mx_row_bytes(fmt, k_pad);
+  if (spread)  // 16 codes of 8 bytes become 16 bytes of shared memory; coordinates count codes
+    return make_tma_2d(map, CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, codes, (uint64_t)k_pad, (uint64_t)rows, row_bytes,
+                       128, (uint32_t)box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
+  return make_tma_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, codes, row_bytes, (uint64_t)rows, row_bytes, 128,
+                     (uint32_t)box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+int make_scale_map(CUtensorMap* map, const void* scales, int fmt, int rows, int k_pad, int box_tiles, int box_blocks) {
+  const uint64_t tiles = (uint64_t)k_pad / mx_block(fmt) / 4;
+  const uint64_t dims[3] = {128, tiles, (uint64_t)mx_rows_pad(rows) / 128};
+  const uint64_t strides[2] = {512, tiles * 512};
+  const uint32_t box[3] = {128, (uint32_t)box_tiles, (uint32_t)box_blocks};
+  return make_tma(map, CU_TENSOR_MAP_DATA_TYPE_INT32, scales, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+
+namespace {
+
+constexpr int kRows = 128;       // weight rows per tile
+constexpr int kMaxStages = 12;
+constexpr int kSplitThreads = 192;
+constexpr int kMaxSplit = 8;
+
+struct SplitBars {
+  uint64_t full[kMaxStages];
+  uint64_t empty[kMaxStages];
+  uint64_t done;
+  uint32_t tmem_base;
+  int abort_flag;
+};
+
+struct SplitArgs {
+  MxOutput o;
+  int steps;    // stages of K in all
+  int split;    // CTAs of the cluster, a share of K each
+  int stages;   // ring depth
+  int n_tiles;  // tiles along the weight's rows
+  int* err;
+};
+
+enum : int { kWaitSplitEmpty = 0x501, kWaitSplitFull = 0x511, kWaitSplitDone = 0x512, kWaitSplitEpi = 0x521 };
+
+template <int MODE, int TN>
+struct SplitShape {
+  static constexpr int kScale = MxMode<MODE>::kScaleTiles * 512;
+  static constexpr int kTok = kRows * 128;            // offset of the tokens' codes in a stage
+  static constexpr int kScaleW = kTok + TN * 128;
+  static constexpr int kScaleT = kScaleW + kScale;
+  static constexpr int kBytes = kScaleT + kScale;
+  // a spread box counts the bytes of its codes, not the padding that it skips
+  static constexpr int kTx = kBytes - (MODE == kModeW4A8 ? kRows * 64 : 0);
+  static constexpr int kStage = (kBytes + 1023) / 1024 * 1024;
+  static constexpr int kSfw = TN < 32 ? 32 : TN;       // columns of tensor memory
+  static constexpr int kSft = kSfw + 4 * MxMode<MODE>::kScaleTiles;
+  static constexpr int kCols = kSft + 4 * MxMode<MODE>::kScaleTiles <= 64 ? 64 : kSft + 16 <= 128 ? 128 : 256;
+};
+
+template <int MODE, int TN>
+__global__ void __launch_bounds__(kSplitThreads)
+    mx_gemm_split_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap t_map,
+                         const __grid_constant__ CUtensorMap sw_map, const __grid_constant__ CUtensorMap st_map,
+                         const __grid_constant__ SplitArgs a) {
+  using S = SplitShape<MODE, TN>;
+  using Mode = MxMode<MODE>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t pad = (1024u - (raw & 1023u)) & 1023u;
+  const uint32_t base = raw + pad;
+  SplitBars* bars = reinterpret_cast<SplitBars*>(smem_raw + pad + (size_t)a.stages * S::kStage);
+  volatile int* abort_flag = &bars->abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = a.split > 1 ? (int)cluster_ctarank() : 0;
+  const int tile = blockIdx.x / a.split;
+  const int n0 = (tile % a.n_tiles) * kRows, m0 = (tile / a.n_tiles) * TN;
+  const int s0 = (int)((int64_t)a.steps * rank / a.split), s1 = (int)((int64_t)a.steps * (rank + 1) / a.split);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < a.stages; ++s) {
+      mbar_init(smem_u32(&bars->full[s]), 1);
+      mbar_init(smem_u32(&bars->empty[s]), 1);
+    }
+    mbar_init(smem_u32(&bars->done), 1);
+    bars->abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 4 && lane == 0) {
+    prefetch_tma_desc(&w_map);
+    prefetch_tma_desc(&t_map);
+    prefetch_tma_desc(&sw_map);
+    prefetch_tma_desc(&st_map);
+  }
+  if (warp == 5) {
+    tmem_alloc_1(smem_u32(&bars->tmem_base), S::kCols);
+    tmem_relinquish_1();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars->tmem_base;
+  pdl_wait();
+  pdl_trigger();
+
+  if (warp == 4) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      uint32_t filled = 0, par = 0;
+      bool ok = true;
+      for (int s = s0; s < s1; ++s) {
+        if (!(ok = mbar_spin_wait(smem_u32(&bars->empty[stage]), phase ^ 1u, abort_flag, a.err, kWaitSplitEmpty))) break;
+        const uint32_t bar = smem_u32(&bars->full[stage]), at = base + (uint32_t)(stage * S::kStage);
+        mbar_arrive_expect_tx(bar, S::kTx);
+        tma_load_2d(at, &w_map, bar, s * 128, n0);
+        tma_load_3d(at + S::kScaleW, &sw_map, bar, 0, s * Mode::kScaleTiles, n0 / 128);
+        tma_load_2d(at + S::kTok, &t_map, bar, s * 128, m0);
+        tma_load_3d(at + S::kScaleT, &st_map, bar, 0, s * Mode::kScaleTiles, m0 / 128);
+        filled |= 1u << stage;
+        par = (par & ~(1u << stage)) | (phase << stage);
+        if (++stage == a.stages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      if (!ok)  // copies in flight land before the CTA exits
+        for (int s = 0; s < a.stages; ++s)
+          if (filled & (1u << s)) mbar_wait_drain(smem_u32(&bars->full[s]), (par >> s) & 1u, 100000000ull);
+    }
+  } else if (warp == 5) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int s = s0; s < s1; ++s) {
+        if (!(ok = mbar_spin_wait(smem_u32(&bars->full[stage]), phase, abort_flag, a.err, kWaitSplitFull))) break;
+        tc_fence_after();
+        const uint32_t at = base + (uint32_t)(stage * S::kStage);
+#pragma unroll
+        for (int t = 0; t < Mode::kScaleTiles; ++t) {
+          copy_scale_tile<false>(tmem + S::kSfw + 4 * t, at + S::kScaleW + 512 * t);
+          copy_scale_tile<false>(tmem + S::kSft + 4 * t, at + S::kScaleT + 512 * t);
+        }
+        const uint64_t dw = desc_k_sw128(at), dt = desc_k_sw128(at + S::kTok);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          umma_mx<MODE, false>(tmem, dw + (uint64_t)(2 * j), dt + (uint64_t)(2 * j),
+                               mx_idesc<MODE>(kRows, TN, true, Mode::byte_of(j)), tmem + S::kSfw + 4 * Mode::tile_of(j),
+                               tmem + S::kSft + 4 * Mode::tile_of(j), (s > s0 || j > 0) ? 1u : 0u);
+        umma_commit_1(smem_u32(&bars->empty[stage]));
+        if (++stage == a.stages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      umma_commit_1(smem_u32(&bars->done));  // also after an abort: MMAs end before TMEM is freed
+      if (!mbar_wait_drain(smem_u32(&bars->done), 0, 1000000000ull)) {
+        *abort_flag = 1;
+        atomicCAS(a.err, 0, kWaitSplitDone);
+      }
+    }
+  }
+  // epilogue: warp w holds weight rows 32 w .. 32 w + 31, one per lane, and every token's column
+  const int row = warp * 32 + lane, n = n0 + row;
+  bool ok = true;
+  if (warp < 4) {
+    ok = mbar_spin_wait(smem_u32(&bars->done), 0, abort_flag, a.err, kWaitSplitEpi) && !*abort_flag;
+    tc_fence_after();
+  }
+  const float alpha = mx_alpha(a.o);
+  const float bias = a.o.bias && warp < 4 && n < a.o.N ? __bfloat162float(a.o.bias[n]) : 0.0f;
+  if (warp < 4) {
+#pragma unroll
+    for (int c = 0; c < TN; c += 16) {
+      if (m0 + c >= a.o.M) break;
+      uint32_t v[16];
+      tmem_ld16(tmem + ((uint32_t)(warp * 32) << 16) + (uint32_t)c, v);
+      tmem_ld_wait_regs16(v);
+      if (!ok) continue;
+      if (a.split > 1) {  // the ring is idle: the partial tile, one token after the other
+        float* part = reinterpret_cast<float*>(smem_raw + pad);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) part[(c + i) * kRows + row] = __uint_as_float(v[i]);
+      } else if (n < a.o.N) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (m0 + c + i < a.o.M) store_one(a.o, m0 + c + i, n, fmaf(alpha, __uint_as_float(v[i]), bias));
+      }
+    }
+  }
+  if (a.split > 1) {
+    cluster_sync();
+    if (warp < 4) {
+      const int per = (TN + a.split - 1) / a.split;
+      const int t1 = min(min(TN, (rank + 1) * per), a.o.M - m0);
+      for (int t = rank * per; t < t1; ++t) {
+        float sum = 0.0f;
+        for (int r = 0; r < a.split; ++r) {
+          float p;
+          asm volatile("ld.shared::cluster.f32 %0, [%1];"
+                       : "=f"(p)
+                       : "r"(mapa_shared(base + (uint32_t)(t * kRows + row) * 4, (uint32_t)r))
+                       : "memory");
+          sum += p;
+        }
+        if (ok && n < a.o.N) store_one(a.o, m0 + t, n, fmaf(alpha, sum, bias));
+      }
+    }
+    cluster_sync();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 5) {
+    tc_fence_after();
+    tmem_dealloc_1(tmem, S::kCols);
+  }
+}
+
+template <int MODE, int TN>
+int launch_split(const MxGemm& g) {
+  using S = SplitShape<MODE, TN>;
+  CUtensorMap w, t, sw, st;
+  int e;
+  const bool spread = MODE == kModeW4A8;
+  if ((e = make_code_map(&w, g.w_codes, g.w_fmt, spread, g.o.N, g.k_pad, kRows))) return e;
+  if ((e = make_code_map(&t, g.a_codes, g.a_fmt, false, g.o.M, g.k_pad, TN))) return e;
+  if ((e = make_scale_map(&sw, g.w_scales, g.w_fmt, g.o.N, g.k_pad, MxMode<MODE>::kScaleTiles, 1))) return e;
+  if ((e = make_scale_map(&st, g.a_scales, g.a_fmt, g.o.M, g.k_pad, MxMode<MODE>::kScaleTiles, 1))) return e;
+  SplitArgs a{};
+  a.o = g.o;
+  a.err = g.err;
+  a.steps = (g.k_pad + MxMode<MODE>::kStageCols - 1) / MxMode<MODE>::kStageCols;
+  a.n_tiles = (g.o.N + kRows - 1) / kRows;
+  const int tiles = a.n_tiles * ((g.o.M + TN - 1) / TN);
+  const int sms = num_sms();
+  a.split = 1;
+  while (a.split < kMaxSplit && tiles * (a.split + 1) <= 2 * sms && 2 * (a.split + 1) <= a.steps) ++a.split;
+  // two CTAs to an SM where more than one wave's worth of CTAs would otherwise wait
+  const int room = tiles * a.split > sms && S::kStage * 4 <= 108 * 1024 ? 108 * 1024 : 216 * 1024;
+  a.stages = room / S::kStage < kMaxStages ? room / S::kStage : kMaxStages;
+  const size_t smem = (size_t)a.stages * S::kStage + sizeof(SplitBars) + 1024;
+  auto kern = mx_gemm_split_kernel<MODE, TN>;
+  const cudaError_t ce = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
+  if (ce != cudaSuccess) return check_cuda(ce, "svdq_mx_gemm: shared memory attribute");
+  return launch_pdl("svdq_mx_gemm launch", kern, dim3((unsigned)tiles * a.split), dim3(kSplitThreads), smem, g.stream,
+                    a.split, w, t, sw, st, a);
+}
+
+template <int MODE>
+int launch_split_mode(const MxGemm& g) {
+  if (g.o.M <= 16) return launch_split<MODE, 16>(g);
+  if (g.o.M <= 32) return launch_split<MODE, 32>(g);
+  if (g.o.M <= 64) return launch_split<MODE, 64>(g);
+  return launch_split<MODE, 128>(g);
+}
+
+}  // namespace
+
+int launch_mx_gemm_split(const MxGemm& g) {
+  if (g.mode == kModeNvfp4) return launch_split_mode<kModeNvfp4>(g);
+  if (g.mode == kModeMxfp4) return launch_split_mode<kModeMxfp4>(g);
+  return launch_split_mode<kModeW4A8>(g);
+}
+
+}  // namespace svdq
+
+extern "C" int svdq_mx_gemm(const void* a_codes, const void* a_scales, int a_format, const float* a_tensor_scale,
+                            const void* w_codes, const void* w_scales, int w_format, const float* w_tensor_scale,
+                            const void* bias, void* out, int out_dtype, int64_t ldo, int M, int N, int K,
+                            cudaStream_t stream) {
+  using namespace svdq;
+  SVDQ_REQUIRE((a_format == w_format && (a_format == kNvfp4 || a_format == kMxfp4)) ||
+                   (a_format == kMxfp8 && w_format == kMxfp4),
+               "svdq_mx_gemm: operands are nvfp4 x nvfp4, mxfp4 x mxfp4 or mxfp8 x mxfp4 (activations x weight)");
+  SVDQ_REQUIRE(dtype_ok(out_dtype), "svdq_mx_gemm: out must be bf16, fp16 or fp32");
+  SVDQ_REQUIRE(M >= 0 && N > 0 && K > 0 && ldo >= N, "svdq_mx_gemm: bad M/N/K/ldo");
+  SVDQ_REQUIRE((!a_tensor_scale && !w_tensor_scale) || a_format == kNvfp4,
+               "svdq_mx_gemm: only nvfp4 operands have tensor scales");
+  if (M == 0) return SVDQ_OK;
+  SVDQ_REQUIRE(a_codes && a_scales && w_codes && w_scales && out, "svdq_mx_gemm: null pointer");
+  SVDQ_REQUIRE(((reinterpret_cast<uintptr_t>(a_codes) | reinterpret_cast<uintptr_t>(a_scales) |
+                 reinterpret_cast<uintptr_t>(w_codes) | reinterpret_cast<uintptr_t>(w_scales)) & 31u) == 0,
+               "svdq_mx_gemm: codes and scales must be 32-byte aligned");
+  SVDQ_REQUIRE((reinterpret_cast<uintptr_t>(out) % dtype_bytes(out_dtype)) == 0 &&
+                   (reinterpret_cast<uintptr_t>(bias) & 1u) == 0,
+               "svdq_mx_gemm: out and bias must be aligned to their elements");
+  if (M > (1 << 24) || N > (1 << 24) || K > (1 << 28))
+    return set_error(SVDQ_ERR_UNSUPPORTED, "svdq_mx_gemm: M and N up to 2^24, K up to 2^28");
+  MxGemm g{};
+  g.mode = a_format == kNvfp4 ? kModeNvfp4 : a_format == kMxfp4 ? kModeMxfp4 : kModeW4A8;
+  g.a_codes = a_codes;
+  g.a_scales = a_scales;
+  g.w_codes = w_codes;
+  g.w_scales = w_scales;
+  g.a_fmt = a_format;
+  g.w_fmt = w_format;
+  g.k_pad = mx_k_pad(K);
+  g.o = MxOutput{a_tensor_scale, w_tensor_scale, static_cast<const __nv_bfloat16*>(bias), out, ldo, out_dtype, M, N};
+  g.stream = stream;
+  g.err = device_error_word();
+  if (!g.err) return set_error(SVDQ_ERR_CUDA, "svdq_mx_gemm: device error word unavailable");
+  return launch_mx_gemm_split(g);
+}

@@ -1,0 +1,306 @@
+// Quantisation to the block-scaled formats, reading them back, and the nvfp4 tensor scale.
+#include "mx_common.cuh"
+
+namespace svdq {
+namespace {
+
+constexpr int kThreads = 256;
+
+// Quotient and remainder by a divisor that is fixed for a launch: floor(n / d) = (n * mul) >> 32 >>
+// shift with mul = ceil(2^(32 + shift) / d), exact for n < 2^31 (T. Granlund, P. Montgomery,
+// "Division by Invariant Integers using Multiplication", PLDI 1994).
+struct FastDiv {
+  uint32_t d, mul, shift;
+};
+FastDiv fast_div(uint32_t d) {
+  uint32_t shift = 0;
+  while ((1u << shift) < d) ++shift;
+  const uint64_t mul = d == 1 ? 0 : (((uint64_t)1 << (31 + shift)) + d - 1) / d;
+  return FastDiv{d, (uint32_t)mul, shift};
+}
+__device__ __forceinline__ uint32_t div_by(const FastDiv& f, uint32_t n) {
+  return f.d == 1 ? n : __umulhi(n, f.mul) >> (f.shift - 1);
+}
+
+struct QuantArgs {
+  const void* x;
+  int64_t ldx;
+  int M, K;
+  int rows;            // rows with scales: M rounded up to 128
+  uint32_t chunks;     // rows * chunks per row
+  FastDiv per_row;     // 16-column chunks per row, K_pad / 16
+  bool vec;
+  const float* tensor_scale;
+  uint8_t* codes;
+  uint8_t* scales;
+};
+
+// One thread quantises 16 columns of a row: a whole nvfp4 block, or half an mx block whose other
+// half is the neighbouring lane's.  Bound by HBM: 2 bytes read and 0.56 written per element from
+// bf16 to nvfp4.  The four scale bytes of a 32-bit word of the tile layout come from 4 (nvfp4) or 8
+// (mx) neighbouring lanes and leave as one store.
+template <typename T, int FMT>
+__global__ void __launch_bounds__(kThreads) mx_quantize_kernel(const QuantArgs a) {
+  pdl_wait();
+  pdl_trigger();
+  const uint32_t id = blockIdx.x * kThreads + threadIdx.x;
+  const int lane = threadIdx.x & 31;
+  const uint32_t row_u = div_by(a.per_row, id);
+  const int row = (int)row_u, chunk = (int)(id - row_u * a.per_row.d);
+  const bool live = id < a.chunks && row < a.M;
+  float v[16];
+  uint32_t amax = 0;
+  {
+    T x[16];
+    if (live) {
+      load_cols<T, 16>(static_cast<const T*>(a.x) + (size_t)row * a.ldx, chunk * 16, a.K, a.vec, x);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] = from_float<T>(0.0f);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      v[i] = to_float(x[i]);
+      amax = max(amax, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+    }
+  }
+  if (FMT != kNvfp4) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+  uint32_t byte = 0;
+  if (live) {
+    const size_t code_row = (size_t)row * mx_row_bytes(FMT, (int)a.per_row.d * 16);
+    if constexpr (FMT == kNvfp4) {
+      const float g = a.tensor_scale ? *a.tensor_scale : 1.0f;
+      byte = nvfp4_scale_byte(amax, g);
+      *reinterpret_cast<uint2*>(a.codes + code_row + chunk * 8) = nvfp4_codes<sizeof(T) == 2>(v, amax, byte, g);
+    } else {
+      byte = mx_scale_byte<FMT>(amax);
+      const float inv = mx_inverse_scale(byte);
+      if (byte == 255u) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = 0.0f;
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] *= inv;
+      if constexpr (FMT == kMxfp4) {
+        *reinterpret_cast<uint2*>(a.codes + code_row + chunk * 8) =
+            make_uint2(e2m1x8_satfinite(v), e2m1x8_satfinite(v + 8));
+      } else {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          w[i] = e4m3x2_satfinite(v[4 * i], v[4 * i + 1]) | e4m3x2_satfinite(v[4 * i + 2], v[4 * i + 3]) << 16;
+        *reinterpret_cast<uint4*>(a.codes + code_row + chunk * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+  }
+  constexpr int kStep = FMT == kNvfp4 ? 1 : 2;  // lanes per block
+  uint32_t word = byte << (8 * ((lane / kStep) & 3));
+  word |= __shfl_xor_sync(0xffffffffu, word, kStep);
+  word |= __shfl_xor_sync(0xffffffffu, word, 2 * kStep);
+  if (id < a.chunks && lane % (4 * kStep) == 0)
+    *reinterpret_cast<uint32_t*>(a.scales + mx_scale_word(row, chunk / (4 * kStep), (int)a.per_row.d / (4 * kStep))) =
+        word;
+}
+
+struct ReadArgs {
+  const uint8_t* codes;
+  const uint8_t* scales;
+  const float* tensor_scale;
+  int M, K;
+  uint32_t chunks;
+  FastDiv per_row;
+  bool vec;
+  void* out;
+  int64_t ldo;
+};
+
+// Reading back: one thread turns 16 codes into values, code * scale (* tensor scale) in fp32,
+// rounded once to T.  Bound by HBM (0.56 bytes read, 2 written per element from nvfp4 to bf16).
+template <typename T, int FMT>
+__global__ void __launch_bounds__(kThreads) mx_dequantize_kernel(const ReadArgs a) {
+  pdl_wait();
+  pdl_trigger();
+  const uint32_t id = blockIdx.x * kThreads + threadIdx.x;
+  if (id >= a.chunks) return;
+  const uint32_t row_u = div_by(a.per_row, id);
+  const int row = (int)row_u, chunk = (int)(id - row_u * a.per_row.d);
+  const int blocks = (int)a.per_row.d * 16 / mx_block(FMT);
+  const int block = chunk * 16 / mx_block(FMT);
+  const uint32_t byte = a.scales[mx_scale_word(row, block >> 2, blocks >> 2) + (block & 3)];
+  float unit;
+  if constexpr (FMT == kNvfp4)
+    unit = e4m3_value(byte) * (a.tensor_scale ? *a.tensor_scale : 1.0f);
+  else
+    unit = e8m0_value(byte);
+  const uint8_t* src = a.codes + (size_t)row * mx_row_bytes(FMT, (int)a.per_row.d * 16);
+  T v[16];
+  if constexpr (FMT == kMxfp8) {
+    const uint4 w = *reinterpret_cast<const uint4*>(src + chunk * 16);
+    const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      uint32_t h2;
+      asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"((uint16_t)(ww[i >> 1] >> (16 * (i & 1)))));
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h2));
+      v[2 * i] = from_float<T>(f.x * unit);
+      v[2 * i + 1] = from_float<T>(f.y * unit);
+    }
+  } else {
+    const uint2 w = *reinterpret_cast<const uint2*>(src + chunk * 8);
+    const uint32_t ww[2] = {w.x, w.y};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      uint32_t h2;
+      asm("{\n\t.reg .b8 b, c;\n\tmov.b16 {b, c}, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, b;\n\t}"
+          : "=r"(h2)
+          : "h"((uint16_t)((ww[i >> 2] >> (8 * (i & 3))) & 0xFFu)));
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h2));
+      v[2 * i] = from_float<T>(f.x * unit);
+      v[2 * i + 1] = from_float<T>(f.y * unit);
+    }
+  }
+  store_cols<T, 16>(static_cast<T*>(a.out) + (size_t)row * a.ldo, chunk * 16, a.K, a.vec, v);
+}
+
+// Largest magnitude of a matrix as fp32 bits, by an integer maximum: any order gives the same
+// result, and a NaN is larger than every number.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) mx_amax_kernel(const T* x, int64_t ldx, uint32_t chunks, FastDiv per_row,
+                                                           int K, bool vec, uint32_t* out) {
+  uint32_t amax = 0;
+  for (uint64_t i = (uint64_t)blockIdx.x * kThreads + threadIdx.x; i < chunks; i += (uint64_t)gridDim.x * kThreads) {
+    const uint32_t row = div_by(per_row, (uint32_t)i);
+    T v[16];
+    load_cols<T, 16>(x + (size_t)row * ldx, (int)((uint32_t)i - row * per_row.d) * 16, K, vec, v);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) amax = max(amax, __float_as_uint(to_float(v[j])) & 0x7FFFFFFFu);
+  }
+  amax = __reduce_max_sync(0xffffffffu, amax);
+  if ((threadIdx.x & 31) == 0) atomicMax(out, amax);
+}
+// amax bits -> the tensor scale amax / (6 * 448), 1 for a matrix of zeros.
+__global__ void mx_tensor_scale_kernel(float* out) {
+  const float amax = *out;
+  *out = amax == 0.0f ? 1.0f : amax / 2688.0f;
+}
+
+// chunks and per_row of an [M, K] matrix padded to K_pad columns; false where a launch cannot hold it
+bool chunk_grid(int rows, int K, uint32_t* chunks, FastDiv* per_row) {
+  const uint32_t per = (uint32_t)mx_k_pad(K) / 16;
+  const uint64_t n = (uint64_t)rows * per;
+  if (n >= (1ull << 31)) return false;
+  *chunks = (uint32_t)n;
+  *per_row = fast_div(per);
+  return true;
+}
+
+template <typename T>
+int launch_quantize(int fmt, const QuantArgs& a, cudaStream_t stream) {
+  const dim3 grid((a.chunks + kThreads - 1) / kThreads);
+  const char* what = "svdq_mx_quantize launch";
+  if (fmt == kNvfp4) return launch_pdl(what, mx_quantize_kernel<T, kNvfp4>, grid, dim3(kThreads), 0, stream, 1, a);
+  if (fmt == kMxfp4) return launch_pdl(what, mx_quantize_kernel<T, kMxfp4>, grid, dim3(kThreads), 0, stream, 1, a);
+  return launch_pdl(what, mx_quantize_kernel<T, kMxfp8>, grid, dim3(kThreads), 0, stream, 1, a);
+}
+template <typename T>
+int launch_dequantize(int fmt, const ReadArgs& a, cudaStream_t stream) {
+  const dim3 grid((a.chunks + kThreads - 1) / kThreads);
+  const char* what = "svdq_mx_dequantize launch";
+  if (fmt == kNvfp4) return launch_pdl(what, mx_dequantize_kernel<T, kNvfp4>, grid, dim3(kThreads), 0, stream, 1, a);
+  if (fmt == kMxfp4) return launch_pdl(what, mx_dequantize_kernel<T, kMxfp4>, grid, dim3(kThreads), 0, stream, 1, a);
+  return launch_pdl(what, mx_dequantize_kernel<T, kMxfp8>, grid, dim3(kThreads), 0, stream, 1, a);
+}
+
+}  // namespace
+}  // namespace svdq
+
+extern "C" size_t svdq_mx_scale_bytes(int rows, int K, int format) {
+  using namespace svdq;
+  if (rows <= 0 || K <= 0 || K > (1 << 30) || rows > (1 << 30) || !mx_format_ok(format)) return 0;
+  return (size_t)mx_rows_pad(rows) * (mx_k_pad(K) / mx_block(format));
+}
+
+extern "C" int svdq_mx_quantize(const void* x, int64_t ldx, int dtype, int M, int K, int format,
+                                const float* tensor_scale, void* codes, void* scales, cudaStream_t stream) {
+  using namespace svdq;
+  SVDQ_REQUIRE(mx_format_ok(format), "svdq_mx_quantize: unknown format");
+  SVDQ_REQUIRE(dtype_ok(dtype), "svdq_mx_quantize: x must be bf16, fp16 or fp32");
+  SVDQ_REQUIRE(M >= 0 && K > 0 && ldx >= K, "svdq_mx_quantize: bad M/K/ldx");
+  SVDQ_REQUIRE(tensor_scale == nullptr || format == kNvfp4, "svdq_mx_quantize: only nvfp4 has a tensor scale");
+  if (M == 0) return SVDQ_OK;
+  SVDQ_REQUIRE(x && codes && scales, "svdq_mx_quantize: null pointer");
+  SVDQ_REQUIRE(((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(scales)) & 15u) == 0,
+               "svdq_mx_quantize: codes and scales must be 16-byte aligned");
+  QuantArgs a{};
+  if (M > (1 << 30) || K > (1 << 30) || !chunk_grid(mx_rows_pad(M), K, &a.chunks, &a.per_row))
+    return set_error(SVDQ_ERR_UNSUPPORTED, "svdq_mx_quantize: more than 2^35 padded elements");
+  a.x = x;
+  a.ldx = ldx;
+  a.M = M;
+  a.K = K;
+  a.rows = mx_rows_pad(M);
+  a.vec = rows_aligned16(x, ldx, dtype_bytes(dtype));
+  a.tensor_scale = tensor_scale;
+  a.codes = static_cast<uint8_t*>(codes);
+  a.scales = static_cast<uint8_t*>(scales);
+  if (dtype == SVDQ_BF16) return launch_quantize<__nv_bfloat16>(format, a, stream);
+  if (dtype == SVDQ_FP16) return launch_quantize<__half>(format, a, stream);
+  return launch_quantize<float>(format, a, stream);
+}
+
+extern "C" int svdq_mx_dequantize(const void* codes, const void* scales, int format, const float* tensor_scale, int M,
+                                  int K, void* out, int64_t ldo, int dtype, cudaStream_t stream) {
+  using namespace svdq;
+  SVDQ_REQUIRE(mx_format_ok(format), "svdq_mx_dequantize: unknown format");
+  SVDQ_REQUIRE(dtype_ok(dtype), "svdq_mx_dequantize: out must be bf16, fp16 or fp32");
+  SVDQ_REQUIRE(M >= 0 && K > 0 && ldo >= K, "svdq_mx_dequantize: bad M/K/ldo");
+  SVDQ_REQUIRE(tensor_scale == nullptr || format == kNvfp4, "svdq_mx_dequantize: only nvfp4 has a tensor scale");
+  if (M == 0) return SVDQ_OK;
+  SVDQ_REQUIRE(codes && scales && out, "svdq_mx_dequantize: null pointer");
+  SVDQ_REQUIRE(((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(scales)) & 15u) == 0,
+               "svdq_mx_dequantize: codes and scales must be 16-byte aligned");
+  ReadArgs a{};
+  if (M > (1 << 30) || K > (1 << 30) || !chunk_grid(M, K, &a.chunks, &a.per_row))
+    return set_error(SVDQ_ERR_UNSUPPORTED, "svdq_mx_dequantize: more than 2^35 padded elements");
+  a.codes = static_cast<const uint8_t*>(codes);
+  a.scales = static_cast<const uint8_t*>(scales);
+  a.tensor_scale = tensor_scale;
+  a.M = M;
+  a.K = K;
+  a.vec = rows_aligned16(out, ldo, dtype_bytes(dtype));
+  a.out = out;
+  a.ldo = ldo;
+  if (dtype == SVDQ_BF16) return launch_dequantize<__nv_bfloat16>(format, a, stream);
+  if (dtype == SVDQ_FP16) return launch_dequantize<__half>(format, a, stream);
+  return launch_dequantize<float>(format, a, stream);
+}
+
+extern "C" int svdq_mx_tensor_scale(const void* x, int64_t ldx, int dtype, int M, int K, float* out,
+                                    cudaStream_t stream) {
+  using namespace svdq;
+  SVDQ_REQUIRE(dtype_ok(dtype), "svdq_mx_tensor_scale: x must be bf16, fp16 or fp32");
+  SVDQ_REQUIRE(M >= 0 && K > 0 && ldx >= K, "svdq_mx_tensor_scale: bad M/K/ldx");
+  SVDQ_REQUIRE(out && (x || M == 0), "svdq_mx_tensor_scale: null pointer");
+  int st = check_cuda(cudaMemsetAsync(out, 0, sizeof(float), stream), "svdq_mx_tensor_scale: clear");
+  if (st) return st;
+  uint32_t chunks = 0;
+  FastDiv per_row{};
+  if (M > (1 << 30) || K > (1 << 30) || !chunk_grid(M, K, &chunks, &per_row))
+    return set_error(SVDQ_ERR_UNSUPPORTED, "svdq_mx_tensor_scale: more than 2^35 padded elements");
+  if (chunks > 0) {
+    const bool vec = rows_aligned16(x, ldx, dtype_bytes(dtype));
+    const uint32_t want = (chunks + kThreads - 1) / kThreads, most = (uint32_t)num_sms() * 8;
+    const dim3 grid(want < most ? want : most), block(kThreads);
+    uint32_t* bits = reinterpret_cast<uint32_t*>(out);
+    if (dtype == SVDQ_BF16)
+      mx_amax_kernel<<<grid, block, 0, stream>>>(static_cast<const __nv_bfloat16*>(x), ldx, chunks, per_row, K, vec, bits);
+    else if (dtype == SVDQ_FP16)
+      mx_amax_kernel<<<grid, block, 0, stream>>>(static_cast<const __half*>(x), ldx, chunks, per_row, K, vec, bits);
+    else
+      mx_amax_kernel<<<grid, block, 0, stream>>>(static_cast<const float*>(x), ldx, chunks, per_row, K, vec, bits);
+    st = check_launch("svdq_mx_tensor_scale launch");
+    if (st) return st;
+  }
+  mx_tensor_scale_kernel<<<1, 1, 0, stream>>>(out);
+  return check_launch("svdq_mx_tensor_scale launch");
+}

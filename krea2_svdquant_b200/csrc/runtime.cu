@@ -94,9 +94,8 @@ int check_launch(const char* what) { return check_cuda(cudaGetLastError(), what)
 static PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
 static std::once_flag g_encode_once;
 
-int make_tma_2d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, uint64_t inner,
-                uint64_t outer, uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer,
-                CUtensorMapSwizzle swizzle) {
+int make_tma(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, int rank, const uint64_t* dims,
+             const uint64_t* strides_bytes, const uint32_t* box, CUtensorMapSwizzle swizzle) {
   std::call_once(g_encode_once, [] {
     void* fn = nullptr;
     cudaDriverEntryPointQueryResult q;
@@ -108,18 +107,31 @@ int make_tma_2d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, u
   if (!g_encode) return set_error(SVDQ_ERR_CUDA, "cuTensorMapEncodeTiled entry point not found");
   if ((reinterpret_cast<uintptr_t>(base) & 15u) != 0)
     return set_error(SVDQ_ERR_INVALID_ARGUMENT, "TMA base address is not 16-byte aligned");
-  if (row_stride_bytes % 16 != 0)
-    return set_error(SVDQ_ERR_INVALID_ARGUMENT, "TMA row stride is not a multiple of 16 bytes");
-  cuuint64_t dims[2] = {inner, outer};
-  cuuint64_t strides[1] = {row_stride_bytes};
-  cuuint32_t box[2] = {box_inner, box_outer};
-  cuuint32_t estr[2] = {1, 1};
-  CUresult r = g_encode(map, dtype, 2, const_cast<void*>(base), dims, strides, box, estr,
+  cuuint64_t gdims[5], gstrides[4];
+  cuuint32_t gbox[5], estr[5];
+  for (int i = 0; i < rank; ++i) {
+    gdims[i] = dims[i];
+    gbox[i] = box[i];
+    estr[i] = 1;
+    if (i == 0) continue;
+    if (strides_bytes[i - 1] % 16 != 0)
+      return set_error(SVDQ_ERR_INVALID_ARGUMENT, "TMA row stride is not a multiple of 16 bytes");
+    gstrides[i - 1] = strides_bytes[i - 1];
+  }
+  CUresult r = g_encode(map, dtype, rank, const_cast<void*>(base), gdims, gstrides, gbox, estr,
                         CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
     return set_error(SVDQ_ERR_CUDA, "cuTensorMapEncodeTiled failed with code " + std::to_string((int)r));
   return SVDQ_OK;
+}
+
+int make_tma_2d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, uint64_t inner,
+                uint64_t outer, uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer,
+                CUtensorMapSwizzle swizzle) {
+  const uint64_t dims[2] = {inner, outer};
+  const uint32_t box[2] = {box_inner, box_outer};
+  return make_tma(map, dtype, base, 2, dims, &row_stride_bytes, box, swizzle);
 }
 
 int num_sms() {

@@ -31,6 +31,10 @@ int make_tma_2d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base,
                 uint64_t inner, uint64_t outer, uint64_t row_stride_bytes,
                 uint32_t box_inner, uint32_t box_outer, CUtensorMapSwizzle swizzle);
 
+// The same for 1 to 5 dimensions (innermost first; strides_bytes has rank - 1 entries).
+int make_tma(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, int rank, const uint64_t* dims,
+             const uint64_t* strides_bytes, const uint32_t* box, CUtensorMapSwizzle swizzle);
+
 // Number of SMs on the current device (cached per device).
 int num_sms();
 

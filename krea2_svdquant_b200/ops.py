@@ -37,6 +37,28 @@ def _stream(dev: torch.device):
     return ctypes.c_void_p(_raw_stream(dev))
 
 
+class _Here:
+    """A ``with`` block that changes nothing."""
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def _on(dev: torch.device):
+    """Makes ``dev`` the current device for a launch: a stream of one device takes no launch while
+    another device is current.  (``torch.cuda.device`` costs several us, so only where it changes
+    something.)"""
+    if dev.index is None or dev.index == torch._C._cuda_getDevice():
+        return _HERE
+    return torch.cuda.device(dev)
+
+
 def _need_cuda(name: str, *ts: Optional[Tensor]) -> None:
     for t in ts:
         if t is not None and not t.is_cuda:
@@ -580,6 +602,205 @@ def w4a4_gemm_narrow(codes8: Tensor, ascales: Tensor, a_group: int, codes: Tenso
 @w4a4_gemm_narrow.register_fake
 def _(codes8, ascales, a_group, codes, scales16, w_group, mid_hl, up_hl, bias, out_fp32):
     return codes8.new_empty((codes8.shape[0], codes.shape[0]), dtype=torch.float32 if out_fp32 else torch.bfloat16)
+
+
+# --------------------------------------------------------------------------- block-scaled formats
+MX_FORMATS = {"nvfp4": _lib.SVDQ_MX_NVFP4, "mxfp4": _lib.SVDQ_MX_MXFP4, "mxfp8": _lib.SVDQ_MX_MXFP8}
+MX_BLOCK = {"nvfp4": 16, "mxfp4": 32, "mxfp8": 32}
+
+
+def mx_k_pad(k: int) -> int:
+    """Columns of a code row: K rounded up to 128."""
+    return (k + 127) // 128 * 128
+
+
+def mx_scales_numel(rows: int, k: int, fmt: str) -> int:
+    """Scale bytes of a [rows, k] matrix: rows rounded up to 128 times the blocks of a code row."""
+    return (rows + 127) // 128 * 128 * (mx_k_pad(k) // MX_BLOCK[fmt])
+
+
+def _mx_codes_like(x: Tensor, rows: int, k: int, fmt: str) -> Tensor:
+    if fmt == "mxfp8":
+        return x.new_empty((rows, mx_k_pad(k)), dtype=torch.float8_e4m3fn)
+    return x.new_empty((rows, mx_k_pad(k) // 2), dtype=torch.uint8)
+
+
+def _mx_check(who: str, codes: Tensor, scales: Tensor, fmt: str, k: int, tensor_scale: Optional[Tensor]) -> None:
+    """A block-scaled operand's tensors: codes of its format and width, every scale, its tensor scale."""
+    _need(fmt in MX_BLOCK, f"{who}: unknown format {fmt!r}; expected one of {sorted(MX_BLOCK)}")
+    want, width = ((torch.float8_e4m3fn, mx_k_pad(k)) if fmt == "mxfp8" else (torch.uint8, mx_k_pad(k) // 2))
+    _need(codes.dtype == want and codes.dim() == 2 and codes.shape[1] == width and codes.is_contiguous(),
+          f"{who}: {fmt} codes must be contiguous {want} [rows, {width}]")
+    _need(scales.dtype == torch.uint8 and scales.dim() == 1 and scales.is_contiguous()
+          and scales.shape[0] == mx_scales_numel(codes.shape[0], k, fmt),
+          f"{who}: scales must be {mx_scales_numel(codes.shape[0], k, fmt)} contiguous bytes in tile order")
+    _mx_check_tensor_scale(who, fmt, tensor_scale)
+
+
+def _mx_check_tensor_scale(who: str, fmt: str, tensor_scale: Optional[Tensor]) -> None:
+    if tensor_scale is not None:
+        _need(fmt == "nvfp4", f"{who}: only nvfp4 has a tensor scale")
+        _need(tensor_scale.dtype == torch.float32 and tensor_scale.numel() == 1,
+              f"{who}: the tensor scale must be one fp32 value")
+
+
+def _same_device(who: str, dev: torch.device, *ts: Optional[Tensor]) -> None:
+    for t in ts:
+        if t is not None and t.device != dev:
+            raise ValueError(f"svdq_b200.{who}: all tensors must be CUDA tensors on one device (got {t.device} and "
+                             f"{dev}); this runtime has no CPU path")
+
+
+def _rows2d(who: str, x: Tensor) -> None:
+    _need(x.dim() == 2 and x.dtype in _DT and x.shape[1] > 0, f"{who}: x must be 2-D bf16, fp16 or fp32 with columns")
+    _need(x.stride(1) == 1 or x.shape[1] == 1, f"{who}: x must have unit column stride")
+
+
+def _ld(x: Tensor) -> int:
+    """Row stride of a 2-D tensor (its width where it has at most one row, whose stride means nothing)."""
+    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+
+
+@_op("mx_quantize")
+def mx_quantize(x: Tensor, fmt: str, tensor_scale: Optional[Tensor]) -> tuple[Tensor, Tensor]:
+    """``x [M, K]`` (bf16, fp16 or fp32, unit column stride) as block-scaled codes and scales
+    (``svdq_mx_quantize``): codes ``[M, K_pad / 2]`` u8 (nvfp4, mxfp4) or ``[M, K_pad]`` e4m3 (mxfp8)
+    and the scale bytes in tile order.  ``tensor_scale``: one fp32 value (nvfp4 only)."""
+    _need_cuda("mx_quantize", x, tensor_scale)
+    _need(fmt in MX_BLOCK, f"mx_quantize: unknown format {fmt!r}; expected one of {sorted(MX_BLOCK)}")
+    _rows2d("mx_quantize", x)
+    _mx_check_tensor_scale("mx_quantize", fmt, tensor_scale)
+    dev = x.device
+    _same_device("mx_quantize", dev, tensor_scale)
+    m, k = x.shape
+    codes = _mx_codes_like(x, m, k, fmt)
+    scales = torch.empty((mx_scales_numel(m, k, fmt),), dtype=torch.uint8, device=dev)
+    if m == 0:
+        return codes, scales
+    with _on(dev):
+        _lib.call("svdq_mx_quantize", x.data_ptr(), _ld(x), _DT[x.dtype], m, k, MX_FORMATS[fmt], _p(tensor_scale),
+                  codes.data_ptr(), scales.data_ptr(), _raw_stream(dev))
+    return codes, scales
+
+
+@mx_quantize.register_fake
+def _(x, fmt, tensor_scale):
+    m, k = x.shape
+    return _mx_codes_like(x, m, k, fmt), x.new_empty((mx_scales_numel(m, k, fmt),), dtype=torch.uint8)
+
+
+@_op("mx_dequantize")
+def mx_dequantize(codes: Tensor, scales: Tensor, fmt: str, k: int, tensor_scale: Optional[Tensor],
+                  dtype: torch.dtype) -> Tensor:
+    """Block-scaled codes and scales read back as ``[M, k]`` of ``dtype``."""
+    _need_cuda("mx_dequantize", codes, scales, tensor_scale)
+    _need(dtype in _DT and k > 0, "mx_dequantize: dtype must be bf16, fp16 or fp32, and k positive")
+    _mx_check("mx_dequantize", codes, scales, fmt, k, tensor_scale)
+    dev = codes.device
+    _same_device("mx_dequantize", dev, scales, tensor_scale)
+    out = torch.empty((codes.shape[0], k), dtype=dtype, device=dev)
+    if codes.shape[0] == 0:
+        return out
+    with _on(dev):
+        _lib.call("svdq_mx_dequantize", codes.data_ptr(), scales.data_ptr(), MX_FORMATS[fmt], _p(tensor_scale),
+                  codes.shape[0], k, out.data_ptr(), k, _DT[dtype], _raw_stream(dev))
+    return out
+
+
+@mx_dequantize.register_fake
+def _(codes, scales, fmt, k, tensor_scale, dtype):
+    return codes.new_empty((codes.shape[0], k), dtype=dtype)
+
+
+@_op("mx_tensor_scale")
+def mx_tensor_scale(x: Tensor) -> Tensor:
+    """The nvfp4 tensor scale ``max |x| / (6 * 448)`` as one fp32 value (1 for zeros)."""
+    _need_cuda("mx_tensor_scale", x)
+    _rows2d("mx_tensor_scale", x)
+    out = torch.empty((1,), dtype=torch.float32, device=x.device)
+    with _on(x.device):
+        _lib.call("svdq_mx_tensor_scale", _p(x), _ld(x), _DT[x.dtype], x.shape[0], x.shape[1], out.data_ptr(),
+                  _raw_stream(x.device))
+    return out
+
+
+@mx_tensor_scale.register_fake
+def _(x):
+    return x.new_empty((1,), dtype=torch.float32)
+
+
+MX_PRODUCTS = (("nvfp4", "nvfp4"), ("mxfp4", "mxfp4"), ("mxfp8", "mxfp4"))  # activations x weight
+
+
+def _mx_gemm_check(who: str, a_fmt: str, w_fmt: str, n: int, bias: Optional[Tensor], out_dtype: torch.dtype) -> None:
+    _need((a_fmt, w_fmt) in MX_PRODUCTS,
+          f"{who}: no product of {a_fmt!r} activations and {w_fmt!r} weights; expected one of {MX_PRODUCTS}")
+    _need(out_dtype in _DT, f"{who}: the output must be bf16, fp16 or fp32")
+    _need(bias is None or (bias.dtype == torch.bfloat16 and bias.is_contiguous() and tuple(bias.shape) == (n,)),
+          f"{who}: bias must be contiguous bf16 [{n}]")
+
+
+@_op("mx_gemm")
+def mx_gemm(a_codes: Tensor, a_scales: Tensor, a_fmt: str, a_tensor_scale: Optional[Tensor], w_codes: Tensor,
+            w_scales: Tensor, w_fmt: str, w_tensor_scale: Optional[Tensor], k: int, bias: Optional[Tensor],
+            out_dtype: torch.dtype) -> Tensor:
+    """``A @ W^T + bias`` of block-scaled matrices ``A [M, k]`` and ``W [N, k]`` on the tensor cores'
+    block-scaled MMAs (``svdq_mx_gemm``); formats as in ``MX_PRODUCTS``, fp32 accumulation."""
+    _need_cuda("mx_gemm", a_codes, a_scales, a_tensor_scale, w_codes, w_scales, w_tensor_scale, bias)
+    _mx_gemm_check("mx_gemm", a_fmt, w_fmt, w_codes.shape[0], bias, out_dtype)
+    _mx_check("mx_gemm (activations)", a_codes, a_scales, a_fmt, k, a_tensor_scale)
+    _mx_check("mx_gemm (weight)", w_codes, w_scales, w_fmt, k, w_tensor_scale)
+    dev = a_codes.device
+    _same_device("mx_gemm", dev, a_scales, a_tensor_scale, w_codes, w_scales, w_tensor_scale, bias)
+    m, n = a_codes.shape[0], w_codes.shape[0]
+    out = torch.empty((m, n), dtype=out_dtype, device=dev)
+    if m == 0 or n == 0:
+        return out
+    with _on(dev):
+        _lib.call("svdq_mx_gemm", a_codes.data_ptr(), a_scales.data_ptr(), MX_FORMATS[a_fmt], _p(a_tensor_scale),
+                  w_codes.data_ptr(), w_scales.data_ptr(), MX_FORMATS[w_fmt], _p(w_tensor_scale), _p(bias),
+                  out.data_ptr(), _DT[out_dtype], n, m, n, k, _raw_stream(dev))
+    return out
+
+
+@mx_gemm.register_fake
+def _(a_codes, a_scales, a_fmt, a_tensor_scale, w_codes, w_scales, w_fmt, w_tensor_scale, k, bias, out_dtype):
+    return a_codes.new_empty((a_codes.shape[0], w_codes.shape[0]), dtype=out_dtype)
+
+
+@_op("rms_norm_mx")
+def rms_norm_mx(x: Tensor, weight: Optional[Tensor], residual: Optional[Tensor],
+                eps: float) -> tuple[Tensor, Tensor, Tensor]:
+    """Root-mean-square norm of ``h = x + residual`` (rounded to x's dtype) as mxfp8 codes and scales
+    (``svdq_rms_norm_mx``); also returns h (empty without a residual, where it is x)."""
+    _need_cuda("rms_norm_mx", x, weight, residual)
+    _rows2d("rms_norm_mx", x)
+    m, h = x.shape
+    dev = x.device
+    _same_device("rms_norm_mx", dev, weight, residual)
+    _need(weight is None or (weight.dtype == x.dtype and tuple(weight.shape) == (h,) and weight.is_contiguous()),
+          f"rms_norm_mx: weight must be contiguous {x.dtype} [{h}]")
+    _need(residual is None or (residual.dtype == x.dtype and residual.shape == x.shape
+                               and (residual.stride(1) == 1 or h == 1)),
+          "rms_norm_mx: residual must have x's shape and dtype and unit column stride")
+    _need(eps >= 0, "rms_norm_mx: eps must not be negative")
+    codes = _mx_codes_like(x, m, h, "mxfp8")
+    scales = torch.empty((mx_scales_numel(m, h, "mxfp8"),), dtype=torch.uint8, device=dev)
+    total = torch.empty((0,) if residual is None else (m, h), dtype=x.dtype, device=dev)
+    if m == 0:
+        return codes, scales, total
+    with _on(dev):
+        _lib.call("svdq_rms_norm_mx", x.data_ptr(), _ld(x), _p(residual), 0 if residual is None else _ld(residual),
+                  _p(weight), _DT[x.dtype], eps, m, h, codes.data_ptr(), scales.data_ptr(), _p(total), h,
+                  _raw_stream(dev))
+    return codes, scales, total
+
+
+@rms_norm_mx.register_fake
+def _(x, weight, residual, eps):
+    m, h = x.shape
+    return (_mx_codes_like(x, m, h, "mxfp8"), x.new_empty((mx_scales_numel(m, h, "mxfp8"),), dtype=torch.uint8),
+            x.new_empty((0,) if residual is None else (m, h)))
 
 
 # The plain implementations of the ops above, same names and arguments.
