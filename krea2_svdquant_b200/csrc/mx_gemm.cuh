@@ -119,5 +119,6 @@ struct MxGemm {
   cudaStream_t stream;
 };
 int launch_mx_gemm_split(const MxGemm& g);
+int launch_mx_gemm_pair(const MxGemm& g);
 
 }  // namespace svdq

@@ -311,5 +311,5 @@ extern "C" int svdq_mx_gemm(const void* a_codes, const void* a_scales, int a_for
   g.stream = stream;
   g.err = device_error_word();
   if (!g.err) return set_error(SVDQ_ERR_CUDA, "svdq_mx_gemm: device error word unavailable");
-  return launch_mx_gemm_split(g);
+  return M > 256 ? launch_mx_gemm_pair(g) : launch_mx_gemm_split(g);
 }
