@@ -195,78 +195,86 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   pdl_wait();
   pdl_trigger();
 
+  // producer and MMA roles: the whole warp runs the loop, one lane issues
   if (warp == 0) {
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0, filled = 0, par = 0;
-      bool ok = true;
-      for (int t = pair; ok && t < a.tiles; t += pairs) {
-        int mb, nb;
-        tile_of(t, a, mb, nb);
-        const int m0 = mb * 2 * BM + (int)rank * BM, n0 = nb * BN + (int)rank * BM;
-        for (int s = 0; s < a.steps; ++s) {
-          if (!(ok = mbar_spin_wait(smem_u32(&bars->empty[stage]), phase ^ 1u, abort_flag, a.err, kWaitPairEmpty)))
-            break;
-          const uint32_t full = mapa_shared(smem_u32(&bars->full[stage]), 0);
-          const uint32_t at = base + (uint32_t)(stage * S::kStage);
+    int stage = 0;
+    uint32_t phase = 0, filled = 0, par = 0;
+    bool ok = true;
+    for (int t = pair; ok && t < a.tiles; t += pairs) {
+      int mb, nb;
+      tile_of(t, a, mb, nb);
+      const int m0 = mb * 2 * BM + (int)rank * BM, n0 = nb * BN + (int)rank * BM;
+      for (int s = 0; s < a.steps; ++s) {
+        if (!(ok = warp_spin_wait(smem_u32(&bars->empty[stage]), phase ^ 1u, abort_flag, a.err, kWaitPairEmpty))) break;
+        const uint32_t full = mapa_shared(smem_u32(&bars->full[stage]), 0);
+        const uint32_t at = base + (uint32_t)(stage * S::kStage);
+        if (elect_one()) {
           if (leader) mbar_arrive_expect_tx(smem_u32(&bars->full[stage]), 2 * S::kTx);
           tma_load_2d_pair(at, &t_map, full, s * 128, m0);
           tma_load_2d_pair(at + S::kB, &w_map, full, s * 128, n0);
           tma_load_3d_pair(at + S::kSfa, &st_map, full, 0, s * S::kTiles, m0 / 128);
           tma_load_3d_pair(at + S::kSfb, &sw_map, full, 0, s * S::kTiles, nb * 2);
-          filled |= 1u << stage;
-          par = (par & ~(1u << stage)) | (phase << stage);
-          if (++stage == S::kStages) {
-            stage = 0;
-            phase ^= 1u;
-          }
+        }
+        __syncwarp();
+        filled |= 1u << stage;
+        par = (par & ~(1u << stage)) | (phase << stage);
+        if (++stage == S::kStages) {
+          stage = 0;
+          phase ^= 1u;
         }
       }
-      if (!ok && leader)  // copies in flight land before the CTA exits
-        for (int s = 0; s < S::kStages; ++s)
-          if (filled & (1u << s)) mbar_wait_drain(smem_u32(&bars->full[s]), (par >> s) & 1u, 100000000ull);
     }
+    if (!ok && leader && lane == 0)  // copies in flight land before the CTA exits
+      for (int s = 0; s < S::kStages; ++s)
+        if (filled & (1u << s)) mbar_wait_drain(smem_u32(&bars->full[s]), (par >> s) & 1u, 100000000ull);
   } else if (warp == 1) {
-    if (lane == 0 && leader) {
+    if (leader) {
       int stage = 0, j = 0;
       uint32_t phase = 0;
       bool ok = true;
+      const uint32_t sfa = tmem + kScaleCol, sfb = sfa + 4 * S::kTiles;
       for (int t = pair; ok && t < a.tiles; t += pairs, ++j) {
-        if (j > 0 && !(ok = mbar_spin_wait(smem_u32(&bars->acc_free), (uint32_t)(j - 1) & 1u, abort_flag, a.err,
+        if (j > 0 && !(ok = warp_spin_wait(smem_u32(&bars->acc_free), (uint32_t)(j - 1) & 1u, abort_flag, a.err,
                                            kWaitPairAcc)))
           break;
         tc_fence_after();
         const uint32_t d = tmem + (uint32_t)((j & 1) * kAccShift);
         for (int s = 0; s < a.steps; ++s) {
-          if (!(ok = mbar_spin_wait(smem_u32(&bars->full[stage]), phase, abort_flag, a.err, kWaitPairFull))) break;
+          if (!(ok = warp_spin_wait(smem_u32(&bars->full[stage]), phase, abort_flag, a.err, kWaitPairFull))) break;
           tc_fence_after();
           const uint32_t at = base + (uint32_t)(stage * S::kStage);
-          const uint32_t sfa = tmem + kScaleCol, sfb = sfa + 4 * S::kTiles;
-#pragma unroll
-          for (int i = 0; i < S::kTiles; ++i) {
-            copy_scale_tile<true>(sfa + 4 * i, at + S::kSfa + 512 * i);
-            copy_scale_tile<true>(sfb + 8 * i, at + S::kSfb + 512 * i);
-            copy_scale_tile<true>(sfb + 8 * i + 4, at + S::kSfb + 512 * (S::kTiles + i));
-          }
           const uint64_t da = desc_k_sw128(at), db = desc_k_sw128(at + S::kB);
+          if (elect_one()) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            umma_mx<MODE, true>(d, da + (uint64_t)(2 * i), db + (uint64_t)(2 * i),
-                                mx_idesc<MODE>(2 * BM, BN, false, Mode::byte_of(i)), sfa + 4 * Mode::tile_of(i),
-                                sfb + 8 * Mode::tile_of(i), (s > 0 || i > 0) ? 1u : 0u);
-          umma_commit_pair(smem_u32(&bars->empty[stage]));
+            for (int i = 0; i < S::kTiles; ++i) {
+              copy_scale_tile<true>(sfa + 4 * i, at + S::kSfa + 512 * i);
+              copy_scale_tile<true>(sfb + 8 * i, at + S::kSfb + 512 * i);
+              copy_scale_tile<true>(sfb + 8 * i + 4, at + S::kSfb + 512 * (S::kTiles + i));
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              umma_mx<MODE, true>(d, da + (uint64_t)(2 * i), db + (uint64_t)(2 * i),
+                                  mx_idesc<MODE>(2 * BM, BN, false, Mode::byte_of(i)), sfa + 4 * Mode::tile_of(i),
+                                  sfb + 8 * Mode::tile_of(i), (s > 0 || i > 0) ? 1u : 0u);
+            umma_commit_pair(smem_u32(&bars->empty[stage]));
+          }
+          __syncwarp();
           if (++stage == S::kStages) {
             stage = 0;
             phase ^= 1u;
           }
         }
-        if (ok) umma_commit_pair(smem_u32(&bars->acc_full[j & 1]));
+        if (ok && elect_one()) umma_commit_pair(smem_u32(&bars->acc_full[j & 1]));
+        __syncwarp();
       }
-      umma_commit_pair_local(smem_u32(&bars->done));  // every MMA ends before TMEM is freed or a CTA exits
-      if (!mbar_wait_drain(smem_u32(&bars->done), 0, 1000000000ull)) {
-        *abort_flag = 1;
-        atomicCAS(a.err, 0, kWaitPairDone);
+      if (elect_one()) {
+        umma_commit_pair_local(smem_u32(&bars->done));  // every MMA ends before TMEM is freed or a CTA exits
+        if (!mbar_wait_drain(smem_u32(&bars->done), 0, 1000000000ull)) {
+          *abort_flag = 1;
+          atomicCAS(a.err, 0, kWaitPairDone);
+        }
       }
+      __syncwarp();
     }
   } else if (warp >= 4) {
     const int half = (warp - 4) >> 2;

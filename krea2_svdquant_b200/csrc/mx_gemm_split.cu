@@ -114,63 +114,67 @@ __global__ void __launch_bounds__(kSplitThreads)
   pdl_wait();
   pdl_trigger();
 
+  // producer and MMA roles: the whole warp runs the loop, one lane issues
   if (warp == 4) {
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      uint32_t filled = 0, par = 0;
-      bool ok = true;
-      for (int s = s0; s < s1; ++s) {
-        if (!(ok = mbar_spin_wait(smem_u32(&bars->empty[stage]), phase ^ 1u, abort_flag, a.err, kWaitSplitEmpty))) break;
-        const uint32_t bar = smem_u32(&bars->full[stage]), at = base + (uint32_t)(stage * S::kStage);
+    int stage = 0;
+    uint32_t phase = 0, filled = 0, par = 0;
+    bool ok = true;
+    for (int s = s0; s < s1; ++s) {
+      if (!(ok = warp_spin_wait(smem_u32(&bars->empty[stage]), phase ^ 1u, abort_flag, a.err, kWaitSplitEmpty))) break;
+      const uint32_t bar = smem_u32(&bars->full[stage]), at = base + (uint32_t)(stage * S::kStage);
+      if (elect_one()) {
         mbar_arrive_expect_tx(bar, S::kTx);
         tma_load_2d(at, &w_map, bar, s * 128, n0);
         tma_load_3d(at + S::kScaleW, &sw_map, bar, 0, s * Mode::kScaleTiles, n0 / 128);
         tma_load_2d(at + S::kTok, &t_map, bar, s * 128, m0);
         tma_load_3d(at + S::kScaleT, &st_map, bar, 0, s * Mode::kScaleTiles, m0 / 128);
-        filled |= 1u << stage;
-        par = (par & ~(1u << stage)) | (phase << stage);
-        if (++stage == a.stages) {
-          stage = 0;
-          phase ^= 1u;
-        }
       }
-      if (!ok)  // copies in flight land before the CTA exits
-        for (int s = 0; s < a.stages; ++s)
-          if (filled & (1u << s)) mbar_wait_drain(smem_u32(&bars->full[s]), (par >> s) & 1u, 100000000ull);
+      __syncwarp();
+      filled |= 1u << stage;
+      par = (par & ~(1u << stage)) | (phase << stage);
+      if (++stage == a.stages) {
+        stage = 0;
+        phase ^= 1u;
+      }
     }
+    if (!ok && lane == 0)  // copies in flight land before the CTA exits
+      for (int s = 0; s < a.stages; ++s)
+        if (filled & (1u << s)) mbar_wait_drain(smem_u32(&bars->full[s]), (par >> s) & 1u, 100000000ull);
   } else if (warp == 5) {
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      for (int s = s0; s < s1; ++s) {
-        if (!(ok = mbar_spin_wait(smem_u32(&bars->full[stage]), phase, abort_flag, a.err, kWaitSplitFull))) break;
-        tc_fence_after();
-        const uint32_t at = base + (uint32_t)(stage * S::kStage);
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int s = s0; s < s1; ++s) {
+      if (!warp_spin_wait(smem_u32(&bars->full[stage]), phase, abort_flag, a.err, kWaitSplitFull)) break;
+      tc_fence_after();
+      const uint32_t at = base + (uint32_t)(stage * S::kStage);
+      const uint64_t dw = desc_k_sw128(at), dt = desc_k_sw128(at + S::kTok);
+      if (elect_one()) {
 #pragma unroll
         for (int t = 0; t < Mode::kScaleTiles; ++t) {
           copy_scale_tile<false>(tmem + S::kSfw + 4 * t, at + S::kScaleW + 512 * t);
           copy_scale_tile<false>(tmem + S::kSft + 4 * t, at + S::kScaleT + 512 * t);
         }
-        const uint64_t dw = desc_k_sw128(at), dt = desc_k_sw128(at + S::kTok);
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           umma_mx<MODE, false>(tmem, dw + (uint64_t)(2 * j), dt + (uint64_t)(2 * j),
                                mx_idesc<MODE>(kRows, TN, true, Mode::byte_of(j)), tmem + S::kSfw + 4 * Mode::tile_of(j),
                                tmem + S::kSft + 4 * Mode::tile_of(j), (s > s0 || j > 0) ? 1u : 0u);
         umma_commit_1(smem_u32(&bars->empty[stage]));
-        if (++stage == a.stages) {
-          stage = 0;
-          phase ^= 1u;
-        }
       }
+      __syncwarp();
+      if (++stage == a.stages) {
+        stage = 0;
+        phase ^= 1u;
+      }
+    }
+    if (elect_one()) {
       umma_commit_1(smem_u32(&bars->done));  // also after an abort: MMAs end before TMEM is freed
       if (!mbar_wait_drain(smem_u32(&bars->done), 0, 1000000000ull)) {
         *abort_flag = 1;
         atomicCAS(a.err, 0, kWaitSplitDone);
       }
     }
+    __syncwarp();
   }
   // epilogue: warp w holds weight rows 32 w .. 32 w + 31, one per lane, and every token's column
   const int row = warp * 32 + lane, n = n0 + row;

@@ -183,6 +183,13 @@ __device__ __forceinline__ bool mbar_spin_wait(uint32_t bar, uint32_t parity, vo
   }
 }
 
+// mbar_spin_wait by a converged warp: every lane gets the same answer, also when some saw the abort
+// flag first, so that the warp stays together.
+__device__ __forceinline__ bool warp_spin_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* err,
+                                               int where) {
+  return __all_sync(0xffffffffu, mbar_spin_wait(bar, parity, abort_flag, err, where));
+}
+
 // Bounded wait for the multi-warp roles: test_wait polls with a short nanosleep between them, so
 // that waiting warps leave the issue slots of their SM sub-partition to the single-thread MMA and
 // TMA roles (a spinning warp takes a share of them; a suspending try_wait is slow to wake).
@@ -236,6 +243,16 @@ __device__ __forceinline__ void cluster_sync() {
 // arrive on an mbarrier given by a shared::cluster address (own CTA or the peer)
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
+// True in one lane of a converged warp (the same one each time).  A role that runs its loop with the
+// whole warp and issues through this keeps its addresses and descriptors in uniform registers,
+// which the TMA and tcgen05 instructions take; in a loop that one lane runs alone every operand is
+// moved there first.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
 }
 
 // ---------------------------------------------------------------------------
