@@ -118,7 +118,6 @@ struct MxGemm {
   int* err;
   cudaStream_t stream;
 };
-int launch_mx_gemm_split(const MxGemm& g);
 int launch_mx_gemm_pair(const MxGemm& g);
 
 }  // namespace svdq

@@ -32,6 +32,7 @@ struct PairBars {
   uint64_t done;
   uint32_t tmem_base;
   int abort_flag;
+  float turn[8][32 * 33];  // a 32 x 32 chunk per epilogue warp, rows padded against bank conflicts
 };
 
 struct PairArgs {
@@ -59,7 +60,8 @@ struct PairShape {
   // of one CTA; a spread box counts the bytes of its codes
   static constexpr int kTx = kBytes - (MODE == kModeW4A8 ? BM * 64 : 0);
   static constexpr int kStage = (kBytes + 1023) / 1024 * 1024;
-  static constexpr int kStages = (225 * 1024) / kStage < kMaxStages ? (225 * 1024) / kStage : kMaxStages;
+  static constexpr int kRing = 227 * 1024 - 1024 - (int)sizeof(PairBars);
+  static constexpr int kStages = kRing / kStage < kMaxStages ? kRing / kStage : kMaxStages;
   static constexpr size_t kSmem = (size_t)kStages * kStage + sizeof(PairBars) + 1024;
 };
 
@@ -97,14 +99,16 @@ __device__ __forceinline__ void store32(void* p, const uint32_t (&w)[8]) {
                : "memory");
 }
 
-// 32 columns of one output row from the accumulator.
-__device__ __forceinline__ void store_chunk(const MxOutput& o, int m, int n, const uint32_t (&acc)[32], float alpha,
-                                            bool wide) {
-  if (m >= o.M || n >= o.N) return;
-  float v[32];
-#pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = alpha * __uint_as_float(acc[i]);
+// 32 x 32 outputs from the accumulator: lane l holds row m0 + l, columns n .. n + 31.  Where the
+// rows allow it each lane writes its row in 32-byte pieces; otherwise (N or the output's address
+// is not a multiple of 32 bytes, or columns are missing) the chunk is turned in shared memory and
+// each row leaves as 32 neighbouring elements.
+__device__ __forceinline__ void store_chunk(const MxOutput& o, int m0, int lane, int n, const uint32_t (&acc)[32],
+                                            float alpha, bool wide, float* turn) {
+  if (m0 >= o.M || n >= o.N) return;
   if (wide && n + 32 <= o.N) {
+    if (m0 + lane >= o.M) return;
+    float v[32];
     if (o.bias) {
       const uint4* b = reinterpret_cast<const uint4*>(o.bias + n);
 #pragma unroll
@@ -118,9 +122,13 @@ __device__ __forceinline__ void store_chunk(const MxOutput& o, int m, int n, con
               fmaf(alpha, __uint_as_float(acc[8 * i + 2 * j + 1]), __uint_as_float(ww[j] & 0xFFFF0000u));
         }
       }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = alpha * __uint_as_float(acc[i]);
     }
+    const size_t at = (size_t)(m0 + lane) * o.ldo + n;
     if (o.out_dtype == SVDQ_FP32) {
-      float* p = static_cast<float*>(o.out) + (size_t)m * o.ldo + n;
+      float* p = static_cast<float*>(o.out) + at;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         uint32_t w[8];
@@ -129,7 +137,7 @@ __device__ __forceinline__ void store_chunk(const MxOutput& o, int m, int n, con
         store32(p + 8 * i, w);
       }
     } else {
-      uint16_t* p = static_cast<uint16_t*>(o.out) + (size_t)m * o.ldo + n;
+      uint16_t* p = static_cast<uint16_t*>(o.out) + at;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         uint32_t w[8];
@@ -141,10 +149,15 @@ __device__ __forceinline__ void store_chunk(const MxOutput& o, int m, int n, con
     return;
   }
 #pragma unroll
-  for (int i = 0; i < 32; ++i)
-    if (n + i < o.N)
-      store_one(o, m, n + i,
-                o.bias ? fmaf(alpha, __uint_as_float(acc[i]), __bfloat162float(o.bias[n + i])) : v[i]);
+  for (int i = 0; i < 32; ++i) turn[lane * 33 + i] = __uint_as_float(acc[i]);
+  __syncwarp();
+  if (n + lane < o.N) {
+    const float bias = o.bias ? __bfloat162float(o.bias[n + lane]) : 0.0f;
+    const int rows = min(32, o.M - m0);
+#pragma unroll 8
+    for (int r = 0; r < rows; ++r) store_one(o, m0 + r, n + lane, fmaf(alpha, turn[r * 33 + lane], bias));
+  }
+  __syncwarp();
 }
 
 template <int MODE>
@@ -278,7 +291,6 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     }
   } else if (warp >= 4) {
     const int half = (warp - 4) >> 2;
-    const int row = (warp & 3) * 32 + lane;
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t free_bar = mapa_shared(smem_u32(&bars->acc_free), 0);
     const float alpha = mx_alpha(a.o);
@@ -289,7 +301,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     for (int t = pair; t < a.tiles; t += pairs, ++j) {
       int mb, nb;
       tile_of(t, a, mb, nb);
-      const int m = mb * 2 * BM + (int)rank * BM + row, n0 = nb * BN;
+      const int m0 = mb * 2 * BM + (int)rank * BM + (warp & 3) * 32, n0 = nb * BN;
       const int first = (j & 1) ? half : 6 + half;  // the chunk in the columns that the accumulators share
       const uint32_t acc = lanes + (uint32_t)((j & 1) * kAccShift);
       if (!mbar_spin_wait(smem_u32(&bars->acc_full[j & 1]), (uint32_t)(j >> 1) & 1u, abort_flag, a.err, kWaitPairEpi))
@@ -308,7 +320,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           if (lane == 0) mbar_arrive_cluster(free_bar);
         }
         if (c < 3) tmem_ld32(acc + (uint32_t)(((first + 2 * (c + 1)) & 7) * 32), nxt);
-        store_chunk(a.o, m, n0 + ((first + 2 * c) & 7) * 32, cur, alpha, wide);
+        store_chunk(a.o, m0, lane, n0 + ((first + 2 * c) & 7) * 32, cur, alpha, wide, bars->turn[warp - 4]);
       }
     }
   }

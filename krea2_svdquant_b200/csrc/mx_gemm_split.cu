@@ -7,6 +7,9 @@
 // where the tiles leave SMs idle, the CTAs of a cluster take a share of K each and add their fp32
 // partial tiles through distributed shared memory in rank order (the same result every time).
 // 6 warps: 0-3 epilogue, 4 TMA producer, 5 MMA and scale copies.
+#include <algorithm>
+#include <atomic>
+
 #include "mx_gemm.cuh"
 
 namespace svdq {
@@ -34,6 +37,7 @@ constexpr int kRows = 128;       // weight rows per tile
 constexpr int kMaxStages = 12;
 constexpr int kSplitThreads = 192;
 constexpr int kMaxSplit = 8;
+constexpr int kRoomTwo = 108 * 1024, kRoomOne = 216 * 1024;  // bytes of a ring with two CTAs or one to an SM
 
 struct SplitBars {
   uint64_t full[kMaxStages];
@@ -42,6 +46,8 @@ struct SplitBars {
   uint32_t tmem_base;
   int abort_flag;
 };
+
+constexpr int kExtra = sizeof(SplitBars) + 1024;
 
 struct SplitArgs {
   MxOutput o;
@@ -205,22 +211,37 @@ __global__ void __launch_bounds__(kSplitThreads)
     }
   }
   if (a.split > 1) {
+    // a share of the tokens each: a thread adds 4 rows of one token over the ranks, in rank order
+    if (!ok) *abort_flag = 1;
     cluster_sync();
-    if (warp < 4) {
-      const int per = (TN + a.split - 1) / a.split;
-      const int t1 = min(min(TN, (rank + 1) * per), a.o.M - m0);
-      for (int t = rank * per; t < t1; ++t) {
-        float sum = 0.0f;
-        for (int r = 0; r < a.split; ++r) {
-          float p;
-          asm volatile("ld.shared::cluster.f32 %0, [%1];"
-                       : "=f"(p)
-                       : "r"(mapa_shared(base + (uint32_t)(t * kRows + row) * 4, (uint32_t)r))
+    const int per = (TN + a.split - 1) / a.split;
+    const int t1 = min(min(TN, (rank + 1) * per), a.o.M - m0);
+    const int r4 = lane * 4, nn = n0 + r4;
+    const bool good = *abort_flag == 0;
+    float b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) b[i] = a.o.bias && nn + i < a.o.N ? __bfloat162float(a.o.bias[nn + i]) : 0.0f;
+    for (int t = rank * per + warp; t < t1; t += kSplitThreads / 32) {
+      float4 p[kMaxSplit];
+#pragma unroll
+      for (int r = 0; r < kMaxSplit; ++r)
+        if (r < a.split)
+          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                       : "=f"(p[r].x), "=f"(p[r].y), "=f"(p[r].z), "=f"(p[r].w)
+                       : "r"(mapa_shared(base + (uint32_t)(t * kRows + r4) * 4, (uint32_t)r))
                        : "memory");
-          sum += p;
+      float v[4] = {p[0].x, p[0].y, p[0].z, p[0].w};
+#pragma unroll
+      for (int r = 1; r < kMaxSplit; ++r)
+        if (r < a.split) {
+          v[0] += p[r].x;
+          v[1] += p[r].y;
+          v[2] += p[r].z;
+          v[3] += p[r].w;
         }
-        if (ok && n < a.o.N) store_one(a.o, m0 + t, n, fmaf(alpha, sum, bias));
-      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (good && nn + i < a.o.N) store_one(a.o, m0 + t, nn + i, fmaf(alpha, v[i], b[i]));
     }
     cluster_sync();
   }
@@ -232,8 +253,76 @@ __global__ void __launch_bounds__(kSplitThreads)
   }
 }
 
+// Clusters of `split` CTAs with an SM to each CTA that run at once on the current device: an
+// occupancy query per cluster size, cached.  (GPCs of 16 to 18 SMs: 74 pairs, 45 clusters of 3, 33
+// of 4, 26 of 5, 22 of 6, 15 of 7 or 8 on a B200.)
+int resident_clusters(const void* kern, int split, size_t smem) {
+  static std::atomic<int> cache[64][kMaxSplit + 1];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  std::atomic<int>* slot = dev >= 0 && dev < 64 ? &cache[dev][split] : nullptr;
+  int n = slot ? slot->load(std::memory_order_relaxed) : 0;
+  if (n > 0) return n;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)split, 1, 1);
+  cfg.blockDim = dim3(kSplitThreads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)split;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n <= 0) {
+    (void)cudaGetLastError();
+    n = num_sms() / split;
+  }
+  if (slot) slot->store(n, std::memory_order_relaxed);
+  return n;
+}
+
+// How a call would run here, and about how long (us past the fixed cost of a launch).
+struct SplitPlan {
+  int steps, n_tiles, tiles, split, stages;
+  float us;
+};
+
+// us per stage of one CTA, [mode][TN]: a stage is 19 to 37 KB through L2 at some 80 GB/s to an SM;
+// nvfp4 at 128 tokens is bound by its scale copies.  Measured at N 6144, K 6144 with one CTA a tile.
+constexpr float kStageUs[3][4] = {{.30f, .33f, .44f, .64f}, {.26f, .28f, .38f, .50f}, {.24f, .26f, .36f, .43f}};
+
 template <int MODE, int TN>
-int launch_split(const MxGemm& g) {
+int plan_split(const MxGemm& g, SplitPlan* p) {
+  using S = SplitShape<MODE, TN>;
+  auto kern = mx_gemm_split_kernel<MODE, TN>;
+  cudaError_t ce = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kRoomOne + kExtra);
+  if (ce == cudaSuccess)
+    ce = cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+  if (ce != cudaSuccess) return check_cuda(ce, "svdq_mx_gemm: shared memory attribute");
+  // two CTAs to an SM where the ring is deep enough at half the memory
+  const int per_sm = S::kStage * 4 <= kRoomTwo ? 2 : 1;
+  p->stages = std::min(kMaxStages, (per_sm == 2 ? kRoomTwo : kRoomOne) / S::kStage);
+  p->steps = (g.k_pad + MxMode<MODE>::kStageCols - 1) / MxMode<MODE>::kStageCols;
+  p->n_tiles = (g.o.N + kRows - 1) / kRows;
+  p->tiles = p->n_tiles * ((g.o.M + TN - 1) / TN);
+  // K is split as far as all clusters still run at once, down to two stages each: one round more
+  // cost more than the deeper split saved at every size measured (N 6144, K 16384, 16 tokens, mxfp8
+  // on mxfp4: 14.0 us split 5 ways, 22.1 in 6)
+  p->split = 1;
+  const void* k = reinterpret_cast<const void*>(kern);
+  for (int s = kMaxSplit; s > 1 && p->split == 1; --s)
+    if (2 * s <= p->steps && p->tiles <= per_sm * resident_clusters(k, s, kRoomOne + kExtra)) p->split = s;
+  const int ctas = p->tiles * p->split, sms = num_sms();
+  const int rounds = (ctas + per_sm * sms - 1) / (per_sm * sms);
+  const float share = ctas > sms && per_sm == 2 ? 1.5f : 1.0f;  // two CTAs of an SM share its bandwidth
+  p->us = rounds * share * (float)((p->steps + p->split - 1) / p->split) * kStageUs[MODE][TN == 16 ? 0 : TN == 32 ? 1 : TN == 64 ? 2 : 3] +
+          (p->split > 1 ? TN / 64.0f : 0.0f);
+  return SVDQ_OK;
+}
+
+template <int MODE, int TN>
+int launch_split(const MxGemm& g, const SplitPlan& p) {
   using S = SplitShape<MODE, TN>;
   CUtensorMap w, t, sw, st;
   int e;
@@ -245,39 +334,36 @@ int launch_split(const MxGemm& g) {
   SplitArgs a{};
   a.o = g.o;
   a.err = g.err;
-  a.steps = (g.k_pad + MxMode<MODE>::kStageCols - 1) / MxMode<MODE>::kStageCols;
-  a.n_tiles = (g.o.N + kRows - 1) / kRows;
-  const int tiles = a.n_tiles * ((g.o.M + TN - 1) / TN);
-  const int sms = num_sms();
-  a.split = 1;
-  while (a.split < kMaxSplit && tiles * (a.split + 1) <= 2 * sms && 2 * (a.split + 1) <= a.steps) ++a.split;
-  // two CTAs to an SM where more than one wave's worth of CTAs would otherwise wait
-  const int room = tiles * a.split > sms && S::kStage * 4 <= 108 * 1024 ? 108 * 1024 : 216 * 1024;
-  a.stages = room / S::kStage < kMaxStages ? room / S::kStage : kMaxStages;
-  const size_t smem = (size_t)a.stages * S::kStage + sizeof(SplitBars) + 1024;
-  auto kern = mx_gemm_split_kernel<MODE, TN>;
-  const cudaError_t ce = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
-  if (ce != cudaSuccess) return check_cuda(ce, "svdq_mx_gemm: shared memory attribute");
-  return launch_pdl("svdq_mx_gemm launch", kern, dim3((unsigned)tiles * a.split), dim3(kSplitThreads), smem, g.stream,
-                    a.split, w, t, sw, st, a);
+  a.steps = p.steps;
+  a.n_tiles = p.n_tiles;
+  a.split = p.split;
+  a.stages = p.stages;
+  return launch_pdl("svdq_mx_gemm launch", mx_gemm_split_kernel<MODE, TN>, dim3((unsigned)(p.tiles * p.split)),
+                    dim3(kSplitThreads), (size_t)a.stages * S::kStage + kExtra, g.stream, a.split, w, t, sw, st, a);
 }
 
+// One product: the pair kernel or this one, whichever is estimated to end first.  A tile of the pair
+// kernel costs 0.42 (nvfp4), 0.40 (mxfp4) or 0.36 us (mxfp8 x mxfp4) per stage.  At N 6144, K 6144,
+// mxfp8 on mxfp4: 128 tokens 16.2 us here against 21.2 on pairs, 256 tokens 25.8 against 21.4.
+template <int MODE, int TN>
+int choose(const MxGemm& g) {
+  constexpr float kPairUs[3] = {.42f, .40f, .36f};
+  SplitPlan p;
+  const int e = plan_split<MODE, TN>(g, &p);
+  if (e) return e;
+  const int pairs = num_sms() / 2, tiles = ((g.o.M + 255) / 256) * ((g.o.N + 255) / 256);
+  const float us = (float)((tiles + pairs - 1) / pairs) * p.steps * kPairUs[MODE];
+  return us < p.us ? launch_mx_gemm_pair(g) : launch_split<MODE, TN>(g, p);
+}
 template <int MODE>
-int launch_split_mode(const MxGemm& g) {
-  if (g.o.M <= 16) return launch_split<MODE, 16>(g);
-  if (g.o.M <= 32) return launch_split<MODE, 32>(g);
-  if (g.o.M <= 64) return launch_split<MODE, 64>(g);
-  return launch_split<MODE, 128>(g);
+int choose_tokens(const MxGemm& g) {
+  if (g.o.M <= 16) return choose<MODE, 16>(g);
+  if (g.o.M <= 32) return choose<MODE, 32>(g);
+  if (g.o.M <= 64) return choose<MODE, 64>(g);
+  return choose<MODE, 128>(g);
 }
 
 }  // namespace
-
-int launch_mx_gemm_split(const MxGemm& g) {
-  if (g.mode == kModeNvfp4) return launch_split_mode<kModeNvfp4>(g);
-  if (g.mode == kModeMxfp4) return launch_split_mode<kModeMxfp4>(g);
-  return launch_split_mode<kModeW4A8>(g);
-}
-
 }  // namespace svdq
 
 extern "C" int svdq_mx_gemm(const void* a_codes, const void* a_scales, int a_format, const float* a_tensor_scale,
@@ -315,5 +401,6 @@ extern "C" int svdq_mx_gemm(const void* a_codes, const void* a_scales, int a_for
   g.stream = stream;
   g.err = device_error_word();
   if (!g.err) return set_error(SVDQ_ERR_CUDA, "svdq_mx_gemm: device error word unavailable");
-  return M > 256 ? launch_mx_gemm_pair(g) : launch_mx_gemm_split(g);
+  if (g.mode == kModeNvfp4) return choose_tokens<kModeNvfp4>(g);
+  return g.mode == kModeMxfp4 ? choose_tokens<kModeMxfp4>(g) : choose_tokens<kModeW4A8>(g);
 }
