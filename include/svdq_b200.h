@@ -506,6 +506,17 @@ int svdq_mx_gemm(const void* a_codes, const void* a_scales, int a_format, const 
                  cudaStream_t stream);
 
 /*
+ * svdq_mx_quantize of x [M, K] (dtype, row stride ldx) to a_format, then svdq_mx_gemm with the weight,
+ * in one call.  The activations' codes and scales are written to the workspace (256-byte aligned, at
+ * least svdq_mx_linear_workspace_bytes(); needs no clearing; one call at a time per workspace).
+ */
+size_t svdq_mx_linear_workspace_bytes(int M, int K, int a_format);
+int svdq_mx_linear(const void* x, int64_t ldx, int dtype, int a_format, const float* a_tensor_scale,
+                   const void* w_codes, const void* w_scales, int w_format, const float* w_tensor_scale,
+                   const void* bias, void* out, int out_dtype, int64_t ldo, int M, int N, int K,
+                   void* workspace, size_t workspace_bytes, cudaStream_t stream);
+
+/*
  * Root-mean-square norm with the residual's addition, written as mxfp8:
  *   h = x + residual (rounded to dtype; stored to sum),  y = h * rsqrt(mean(h^2) + eps) * weight,
  *   y quantised to SVDQ_MX_MXFP8 from fp32.

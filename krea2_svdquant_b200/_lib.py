@@ -89,6 +89,9 @@ SIGNATURES = {
     "svdq_mx_tensor_scale": ([c_void_p, c_int64, c_int, c_int, c_int, c_void_p, c_void_p], c_int),
     "svdq_mx_gemm": ([c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
                       c_int, c_int64, c_int, c_int, c_int, c_void_p], c_int),
+    "svdq_mx_linear_workspace_bytes": ([c_int, c_int, c_int], ctypes.c_size_t),
+    "svdq_mx_linear": ([c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
+                        c_void_p, c_int, c_int64, c_int, c_int, c_int, c_void_p, ctypes.c_size_t, c_void_p], c_int),
     "svdq_rms_norm_mx": ([c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, ctypes.c_float, c_int, c_int,
                           c_void_p, c_void_p, c_void_p, c_int64, c_void_p], c_int),
 }

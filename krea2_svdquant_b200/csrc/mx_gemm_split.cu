@@ -404,3 +404,35 @@ extern "C" int svdq_mx_gemm(const void* a_codes, const void* a_scales, int a_for
   if (g.mode == kModeNvfp4) return choose_tokens<kModeNvfp4>(g);
   return g.mode == kModeMxfp4 ? choose_tokens<kModeMxfp4>(g) : choose_tokens<kModeW4A8>(g);
 }
+
+// Workspace of svdq_mx_linear: the codes, then the scales from the next 256-byte boundary.
+static size_t mx_code_bytes(int M, int K, int fmt) {
+  return ((size_t)M * svdq::mx_row_bytes(fmt, svdq::mx_k_pad(K)) + 255) / 256 * 256;
+}
+
+extern "C" size_t svdq_mx_linear_workspace_bytes(int M, int K, int a_format) {
+  if (M <= 0 || K <= 0 || !svdq::mx_format_ok(a_format) || M > (1 << 30) || K > (1 << 30)) return 0;
+  return mx_code_bytes(M, K, a_format) + svdq_mx_scale_bytes(M, K, a_format);
+}
+
+extern "C" int svdq_mx_linear(const void* x, int64_t ldx, int dtype, int a_format, const float* a_tensor_scale,
+                              const void* w_codes, const void* w_scales, int w_format, const float* w_tensor_scale,
+                              const void* bias, void* out, int out_dtype, int64_t ldo, int M, int N, int K,
+                              void* workspace, size_t workspace_bytes, cudaStream_t stream) {
+  using namespace svdq;
+  SVDQ_REQUIRE(mx_format_ok(a_format), "svdq_mx_linear: unknown activation format");
+  SVDQ_REQUIRE(M >= 0 && K > 0, "svdq_mx_linear: bad M/K");
+  SVDQ_REQUIRE(M == 0 || (workspace && (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0 &&
+                          workspace_bytes >= svdq_mx_linear_workspace_bytes(M, K, a_format)),
+               "svdq_mx_linear: workspace must be 256-byte aligned and hold svdq_mx_linear_workspace_bytes()");
+  uint8_t* codes = static_cast<uint8_t*>(workspace);
+  uint8_t* scales = M > 0 ? codes + mx_code_bytes(M, K, a_format) : nullptr;
+  // the product's arguments are checked before anything is launched
+  int st = svdq_mx_gemm(codes, scales, a_format, a_tensor_scale, w_codes, w_scales, w_format, w_tensor_scale, bias, out,
+                        out_dtype, ldo, 0, N, K, stream);
+  if (!st) st = svdq_mx_quantize(x, ldx, dtype, M, K, a_format, a_tensor_scale, codes, scales, stream);
+  if (!st)
+    st = svdq_mx_gemm(codes, scales, a_format, a_tensor_scale, w_codes, w_scales, w_format, w_tensor_scale, bias, out,
+                      out_dtype, ldo, M, N, K, stream);
+  return st;
+}

@@ -56,12 +56,15 @@ class MicroTensor:
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
-    """x [..., K] as 2-D rows with unit column stride (a view where its strides allow one)."""
+    """x [..., K] as 2-D rows with unit column stride that do not overlap (a view where its strides
+    allow one, otherwise a copy: a transposed or an expanded x)."""
     if x.dim() < 1:
         raise ValueError("expected a tensor with at least one dimension")
     if x.dim() != 2:
         x = x.reshape(-1, x.shape[-1])
-    return x if x.stride(1) == 1 or x.shape[1] == 1 else x.contiguous()
+    if x.is_contiguous() or (x.stride(1) == 1 and x.stride(0) >= x.shape[1]):
+        return x
+    return x.contiguous()
 
 
 def tensor_scale(x: torch.Tensor) -> torch.Tensor:
@@ -74,7 +77,7 @@ def quantize(x: torch.Tensor, fmt: str = "nvfp4", *, tensor_scale: torch.Tensor 
     (None: 1); for weights use :func:`tensor_scale`.  Codes are those of the exact quotients, ties to
     even; a block with an infinity or a NaN reads back as NaN."""
     codes, scales = _kernels().mx_quantize(_rows(x), fmt, tensor_scale)
-    return MicroTensor(codes, scales, fmt, tuple(x.shape), tensor_scale)
+    return MicroTensor(codes, scales, fmt, x.shape, tensor_scale)
 
 
 def dequantize(t: MicroTensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
@@ -100,7 +103,11 @@ def linear(x: torch.Tensor | MicroTensor, w: MicroTensor, bias: torch.Tensor | N
     a :class:`MicroTensor` already goes straight to the product (bf16 output by default)."""
     if isinstance(x, MicroTensor):
         return matmul(x, w, bias, out_dtype=out_dtype or torch.bfloat16)
-    return matmul(quantize(x, act, tensor_scale=act_scale), w, bias, out_dtype=out_dtype or x.dtype)
+    if len(w.shape) != 2 or x.dim() < 1 or x.shape[-1] != w.shape[1]:
+        raise ValueError(f"linear: activations {tuple(x.shape)} and weight {w.shape} do not match")
+    out = _kernels().mx_linear(_rows(x), act, act_scale, w.codes, w.scales, w.fmt, w.tensor_scale, bias,
+                               out_dtype or x.dtype)
+    return out if x.dim() == 2 else out.reshape(*x.shape[:-1], w.shape[0])
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, *, residual: torch.Tensor | None = None,
@@ -112,8 +119,11 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, *, residual: t
     if residual is not None and residual.shape != x.shape:
         raise ValueError(f"rms_norm: residual {tuple(residual.shape)} must have x's shape {tuple(x.shape)}")
     codes, scales, total = _kernels().rms_norm_mx(x2, weight, None if residual is None else _rows(residual), eps)
-    return (MicroTensor(codes, scales, "mxfp8", tuple(x.shape)),
-            x if residual is None else total.reshape(x.shape))
+    if residual is None:
+        total = x
+    elif x.dim() != 2:
+        total = total.reshape(x.shape)
+    return MicroTensor(codes, scales, "mxfp8", x.shape), total
 
 
 class MicroscaledLinear(nn.Module):

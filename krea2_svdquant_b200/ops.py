@@ -625,40 +625,65 @@ def _mx_codes_like(x: Tensor, rows: int, k: int, fmt: str) -> Tensor:
     return x.new_empty((rows, mx_k_pad(k) // 2), dtype=torch.uint8)
 
 
-def _mx_check(who: str, codes: Tensor, scales: Tensor, fmt: str, k: int, tensor_scale: Optional[Tensor]) -> None:
-    """A block-scaled operand's tensors: codes of its format and width, every scale, its tensor scale."""
-    _need(fmt in MX_BLOCK, f"{who}: unknown format {fmt!r}; expected one of {sorted(MX_BLOCK)}")
-    want, width = ((torch.float8_e4m3fn, mx_k_pad(k)) if fmt == "mxfp8" else (torch.uint8, mx_k_pad(k) // 2))
-    _need(codes.dtype == want and codes.dim() == 2 and codes.shape[1] == width and codes.is_contiguous(),
-          f"{who}: {fmt} codes must be contiguous {want} [rows, {width}]")
-    _need(scales.dtype == torch.uint8 and scales.dim() == 1 and scales.is_contiguous()
-          and scales.shape[0] == mx_scales_numel(codes.shape[0], k, fmt),
-          f"{who}: scales must be {mx_scales_numel(codes.shape[0], k, fmt)} contiguous bytes in tile order")
-    _mx_check_tensor_scale(who, fmt, tensor_scale)
-
-
-def _mx_check_tensor_scale(who: str, fmt: str, tensor_scale: Optional[Tensor]) -> None:
-    if tensor_scale is not None:
-        _need(fmt == "nvfp4", f"{who}: only nvfp4 has a tensor scale")
-        _need(tensor_scale.dtype == torch.float32 and tensor_scale.numel() == 1,
-              f"{who}: the tensor scale must be one fp32 value")
-
-
-def _same_device(who: str, dev: torch.device, *ts: Optional[Tensor]) -> None:
-    for t in ts:
+# The checks below cost a small call a few us of host time, so they build their messages only to raise.
+def _mx_device(who: str, first: Tensor, *rest: Optional[Tensor]) -> torch.device:
+    """The one CUDA device of the tensors."""
+    dev = first.device
+    for t in rest:
         if t is not None and t.device != dev:
             raise ValueError(f"svdq_b200.{who}: all tensors must be CUDA tensors on one device (got {t.device} and "
                              f"{dev}); this runtime has no CPU path")
+    if dev.type != "cuda":
+        raise ValueError(f"svdq_b200.{who}: all tensors must be CUDA tensors (got {dev}); this runtime has no CPU path")
+    return dev
 
 
-def _rows2d(who: str, x: Tensor) -> None:
-    _need(x.dim() == 2 and x.dtype in _DT and x.shape[1] > 0, f"{who}: x must be 2-D bf16, fp16 or fp32 with columns")
-    _need(x.stride(1) == 1 or x.shape[1] == 1, f"{who}: x must have unit column stride")
+def _mx_format(who: str, fmt: str) -> int:
+    code = MX_FORMATS.get(fmt)
+    if code is None:
+        raise ValueError(f"{who}: unknown format {fmt!r}; expected one of {sorted(MX_BLOCK)}")
+    return code
 
 
-def _ld(x: Tensor) -> int:
-    """Row stride of a 2-D tensor (its width where it has at most one row, whose stride means nothing)."""
-    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+def _mx_check(who: str, codes: Tensor, scales: Tensor, fmt: str, k: int, tensor_scale: Optional[Tensor]) -> int:
+    """Checks a block-scaled operand's tensors (codes of its format and width, every scale, its tensor
+    scale) and returns the format's code."""
+    code = _mx_format(who, fmt)
+    want, width = (torch.float8_e4m3fn, mx_k_pad(k)) if fmt == "mxfp8" else (torch.uint8, mx_k_pad(k) // 2)
+    if codes.dtype != want or codes.dim() != 2 or codes.shape[1] != width or not codes.is_contiguous():
+        raise ValueError(f"{who}: {fmt} codes must be contiguous {want} [rows, {width}], got {codes.dtype} "
+                         f"{tuple(codes.shape)}")
+    if (scales.dtype != torch.uint8 or scales.dim() != 1 or not scales.is_contiguous()
+            or scales.shape[0] != mx_scales_numel(codes.shape[0], k, fmt)):
+        raise ValueError(f"{who}: scales must be {mx_scales_numel(codes.shape[0], k, fmt)} contiguous bytes in tile "
+                         f"order, got {scales.dtype} {tuple(scales.shape)}")
+    if tensor_scale is not None:
+        _mx_check_tensor_scale(who, fmt, tensor_scale)
+    return code
+
+
+def _mx_check_tensor_scale(who: str, fmt: str, tensor_scale: Tensor) -> None:
+    if fmt != "nvfp4":
+        raise ValueError(f"{who}: only nvfp4 has a tensor scale")
+    if tensor_scale.dtype != torch.float32 or tensor_scale.numel() != 1:
+        raise ValueError(f"{who}: the tensor scale must be one fp32 value")
+
+
+def _mx_rows(who: str, x: Tensor) -> tuple[int, int, int]:
+    """(rows, columns, row stride) of a 2-D floating tensor with unit column stride."""
+    if x.dim() != 2 or x.dtype not in _DT:
+        raise ValueError(f"{who}: expected a 2-D bf16, fp16 or fp32 tensor, got {x.dtype} {tuple(x.shape)}")
+    m, k = x.shape
+    if k == 0 or (k > 1 and x.stride(1) != 1):
+        raise ValueError(f"{who}: rows must have columns and unit column stride")
+    ld = x.stride(0) if m > 1 else k  # the stride of a single row means nothing
+    if ld < k:
+        raise ValueError(f"{who}: rows must not overlap (row stride {ld} of {k} columns)")
+    return m, k, ld
+
+
+def _ptr(t: Optional[Tensor]):
+    return None if t is None else t.data_ptr()
 
 
 @_op("mx_quantize")
@@ -666,20 +691,17 @@ def mx_quantize(x: Tensor, fmt: str, tensor_scale: Optional[Tensor]) -> tuple[Te
     """``x [M, K]`` (bf16, fp16 or fp32, unit column stride) as block-scaled codes and scales
     (``svdq_mx_quantize``): codes ``[M, K_pad / 2]`` u8 (nvfp4, mxfp4) or ``[M, K_pad]`` e4m3 (mxfp8)
     and the scale bytes in tile order.  ``tensor_scale``: one fp32 value (nvfp4 only)."""
-    _need_cuda("mx_quantize", x, tensor_scale)
-    _need(fmt in MX_BLOCK, f"mx_quantize: unknown format {fmt!r}; expected one of {sorted(MX_BLOCK)}")
-    _rows2d("mx_quantize", x)
-    _mx_check_tensor_scale("mx_quantize", fmt, tensor_scale)
-    dev = x.device
-    _same_device("mx_quantize", dev, tensor_scale)
-    m, k = x.shape
+    dev = _mx_device("mx_quantize", x, tensor_scale)
+    code = _mx_format("mx_quantize", fmt)
+    m, k, ld = _mx_rows("mx_quantize", x)
+    if tensor_scale is not None:
+        _mx_check_tensor_scale("mx_quantize", fmt, tensor_scale)
     codes = _mx_codes_like(x, m, k, fmt)
-    scales = torch.empty((mx_scales_numel(m, k, fmt),), dtype=torch.uint8, device=dev)
-    if m == 0:
-        return codes, scales
-    with _on(dev):
-        _lib.call("svdq_mx_quantize", x.data_ptr(), _ld(x), _DT[x.dtype], m, k, MX_FORMATS[fmt], _p(tensor_scale),
-                  codes.data_ptr(), scales.data_ptr(), _raw_stream(dev))
+    scales = x.new_empty((mx_scales_numel(m, k, fmt),), dtype=torch.uint8)
+    if m:
+        with _on(dev):
+            _lib.call("svdq_mx_quantize", x.data_ptr(), ld, _DT[x.dtype], m, k, code, _ptr(tensor_scale),
+                      codes.data_ptr(), scales.data_ptr(), _raw_stream(dev))
     return codes, scales
 
 
@@ -693,17 +715,16 @@ def _(x, fmt, tensor_scale):
 def mx_dequantize(codes: Tensor, scales: Tensor, fmt: str, k: int, tensor_scale: Optional[Tensor],
                   dtype: torch.dtype) -> Tensor:
     """Block-scaled codes and scales read back as ``[M, k]`` of ``dtype``."""
-    _need_cuda("mx_dequantize", codes, scales, tensor_scale)
-    _need(dtype in _DT and k > 0, "mx_dequantize: dtype must be bf16, fp16 or fp32, and k positive")
-    _mx_check("mx_dequantize", codes, scales, fmt, k, tensor_scale)
-    dev = codes.device
-    _same_device("mx_dequantize", dev, scales, tensor_scale)
-    out = torch.empty((codes.shape[0], k), dtype=dtype, device=dev)
-    if codes.shape[0] == 0:
-        return out
-    with _on(dev):
-        _lib.call("svdq_mx_dequantize", codes.data_ptr(), scales.data_ptr(), MX_FORMATS[fmt], _p(tensor_scale),
-                  codes.shape[0], k, out.data_ptr(), k, _DT[dtype], _raw_stream(dev))
+    dev = _mx_device("mx_dequantize", codes, scales, tensor_scale)
+    if dtype not in _DT or k <= 0:
+        raise ValueError("mx_dequantize: dtype must be bf16, fp16 or fp32, and k positive")
+    code = _mx_check("mx_dequantize", codes, scales, fmt, k, tensor_scale)
+    m = codes.shape[0]
+    out = codes.new_empty((m, k), dtype=dtype)
+    if m:
+        with _on(dev):
+            _lib.call("svdq_mx_dequantize", codes.data_ptr(), scales.data_ptr(), code, _ptr(tensor_scale), m, k,
+                      out.data_ptr(), k, _DT[dtype], _raw_stream(dev))
     return out
 
 
@@ -715,12 +736,11 @@ def _(codes, scales, fmt, k, tensor_scale, dtype):
 @_op("mx_tensor_scale")
 def mx_tensor_scale(x: Tensor) -> Tensor:
     """The nvfp4 tensor scale ``max |x| / (6 * 448)`` as one fp32 value (1 for zeros)."""
-    _need_cuda("mx_tensor_scale", x)
-    _rows2d("mx_tensor_scale", x)
-    out = torch.empty((1,), dtype=torch.float32, device=x.device)
-    with _on(x.device):
-        _lib.call("svdq_mx_tensor_scale", _p(x), _ld(x), _DT[x.dtype], x.shape[0], x.shape[1], out.data_ptr(),
-                  _raw_stream(x.device))
+    dev = _mx_device("mx_tensor_scale", x)
+    m, k, ld = _mx_rows("mx_tensor_scale", x)
+    out = x.new_empty((1,), dtype=torch.float32)
+    with _on(dev):
+        _lib.call("svdq_mx_tensor_scale", _p(x), ld, _DT[x.dtype], m, k, out.data_ptr(), _raw_stream(dev))
     return out
 
 
@@ -733,11 +753,14 @@ MX_PRODUCTS = (("nvfp4", "nvfp4"), ("mxfp4", "mxfp4"), ("mxfp8", "mxfp4"))  # ac
 
 
 def _mx_gemm_check(who: str, a_fmt: str, w_fmt: str, n: int, bias: Optional[Tensor], out_dtype: torch.dtype) -> None:
-    _need((a_fmt, w_fmt) in MX_PRODUCTS,
-          f"{who}: no product of {a_fmt!r} activations and {w_fmt!r} weights; expected one of {MX_PRODUCTS}")
-    _need(out_dtype in _DT, f"{who}: the output must be bf16, fp16 or fp32")
-    _need(bias is None or (bias.dtype == torch.bfloat16 and bias.is_contiguous() and tuple(bias.shape) == (n,)),
-          f"{who}: bias must be contiguous bf16 [{n}]")
+    if (a_fmt, w_fmt) not in MX_PRODUCTS:
+        raise ValueError(f"{who}: no product of {a_fmt!r} activations and {w_fmt!r} weights; expected one of "
+                         f"{MX_PRODUCTS}")
+    if out_dtype not in _DT:
+        raise ValueError(f"{who}: the output must be bf16, fp16 or fp32")
+    if bias is not None and (bias.dtype != torch.bfloat16 or bias.dim() != 1 or bias.shape[0] != n
+                             or not bias.is_contiguous()):
+        raise ValueError(f"{who}: bias must be contiguous bf16 [{n}]")
 
 
 @_op("mx_gemm")
@@ -746,20 +769,17 @@ def mx_gemm(a_codes: Tensor, a_scales: Tensor, a_fmt: str, a_tensor_scale: Optio
             out_dtype: torch.dtype) -> Tensor:
     """``A @ W^T + bias`` of block-scaled matrices ``A [M, k]`` and ``W [N, k]`` on the tensor cores'
     block-scaled MMAs (``svdq_mx_gemm``); formats as in ``MX_PRODUCTS``, fp32 accumulation."""
-    _need_cuda("mx_gemm", a_codes, a_scales, a_tensor_scale, w_codes, w_scales, w_tensor_scale, bias)
-    _mx_gemm_check("mx_gemm", a_fmt, w_fmt, w_codes.shape[0], bias, out_dtype)
-    _mx_check("mx_gemm (activations)", a_codes, a_scales, a_fmt, k, a_tensor_scale)
-    _mx_check("mx_gemm (weight)", w_codes, w_scales, w_fmt, k, w_tensor_scale)
-    dev = a_codes.device
-    _same_device("mx_gemm", dev, a_scales, a_tensor_scale, w_codes, w_scales, w_tensor_scale, bias)
+    dev = _mx_device("mx_gemm", a_codes, a_scales, a_tensor_scale, w_codes, w_scales, w_tensor_scale, bias)
+    a_code = _mx_check("mx_gemm (activations)", a_codes, a_scales, a_fmt, k, a_tensor_scale)
+    w_code = _mx_check("mx_gemm (weight)", w_codes, w_scales, w_fmt, k, w_tensor_scale)
     m, n = a_codes.shape[0], w_codes.shape[0]
-    out = torch.empty((m, n), dtype=out_dtype, device=dev)
-    if m == 0 or n == 0:
-        return out
-    with _on(dev):
-        _lib.call("svdq_mx_gemm", a_codes.data_ptr(), a_scales.data_ptr(), MX_FORMATS[a_fmt], _p(a_tensor_scale),
-                  w_codes.data_ptr(), w_scales.data_ptr(), MX_FORMATS[w_fmt], _p(w_tensor_scale), _p(bias),
-                  out.data_ptr(), _DT[out_dtype], n, m, n, k, _raw_stream(dev))
+    _mx_gemm_check("mx_gemm", a_fmt, w_fmt, n, bias, out_dtype)
+    out = a_codes.new_empty((m, n), dtype=out_dtype)
+    if m and n:
+        with _on(dev):
+            _lib.call("svdq_mx_gemm", a_codes.data_ptr(), a_scales.data_ptr(), a_code, _ptr(a_tensor_scale),
+                      w_codes.data_ptr(), w_scales.data_ptr(), w_code, _ptr(w_tensor_scale), _ptr(bias),
+                      out.data_ptr(), _DT[out_dtype], n, m, n, k, _raw_stream(dev))
     return out
 
 
@@ -768,31 +788,60 @@ def _(a_codes, a_scales, a_fmt, a_tensor_scale, w_codes, w_scales, w_fmt, w_tens
     return a_codes.new_empty((a_codes.shape[0], w_codes.shape[0]), dtype=out_dtype)
 
 
+@_op("mx_linear")
+def mx_linear(x: Tensor, a_fmt: str, a_tensor_scale: Optional[Tensor], w_codes: Tensor, w_scales: Tensor, w_fmt: str,
+              w_tensor_scale: Optional[Tensor], bias: Optional[Tensor], out_dtype: torch.dtype) -> Tensor:
+    """``mx_gemm(*mx_quantize(x, a_fmt, a_tensor_scale), ...)`` in one call (``svdq_mx_linear``): the
+    activations' codes and scales live in a workspace."""
+    dev = _mx_device("mx_linear", x, a_tensor_scale, w_codes, w_scales, w_tensor_scale, bias)
+    a_code = _mx_format("mx_linear", a_fmt)
+    m, k, ld = _mx_rows("mx_linear", x)
+    if a_tensor_scale is not None:
+        _mx_check_tensor_scale("mx_linear", a_fmt, a_tensor_scale)
+    w_code = _mx_check("mx_linear (weight)", w_codes, w_scales, w_fmt, k, w_tensor_scale)
+    n = w_codes.shape[0]
+    _mx_gemm_check("mx_linear", a_fmt, w_fmt, n, bias, out_dtype)
+    out = x.new_empty((m, n), dtype=out_dtype)
+    if m and n:
+        codes = m * mx_k_pad(k) // (1 if a_fmt == "mxfp8" else 2)
+        ws = x.new_empty((codes + 1024 + mx_scales_numel(m, k, a_fmt),), dtype=torch.uint8)
+        with _on(dev):
+            _lib.call("svdq_mx_linear", x.data_ptr(), ld, _DT[x.dtype], a_code, _ptr(a_tensor_scale),
+                      w_codes.data_ptr(), w_scales.data_ptr(), w_code, _ptr(w_tensor_scale), _ptr(bias),
+                      out.data_ptr(), _DT[out_dtype], n, m, n, k, ws.data_ptr(), ws.shape[0], _raw_stream(dev))
+    return out
+
+
+@mx_linear.register_fake
+def _(x, a_fmt, a_tensor_scale, w_codes, w_scales, w_fmt, w_tensor_scale, bias, out_dtype):
+    return x.new_empty((x.shape[0], w_codes.shape[0]), dtype=out_dtype)
+
+
 @_op("rms_norm_mx")
 def rms_norm_mx(x: Tensor, weight: Optional[Tensor], residual: Optional[Tensor],
                 eps: float) -> tuple[Tensor, Tensor, Tensor]:
     """Root-mean-square norm of ``h = x + residual`` (rounded to x's dtype) as mxfp8 codes and scales
     (``svdq_rms_norm_mx``); also returns h (empty without a residual, where it is x)."""
-    _need_cuda("rms_norm_mx", x, weight, residual)
-    _rows2d("rms_norm_mx", x)
-    m, h = x.shape
-    dev = x.device
-    _same_device("rms_norm_mx", dev, weight, residual)
-    _need(weight is None or (weight.dtype == x.dtype and tuple(weight.shape) == (h,) and weight.is_contiguous()),
-          f"rms_norm_mx: weight must be contiguous {x.dtype} [{h}]")
-    _need(residual is None or (residual.dtype == x.dtype and residual.shape == x.shape
-                               and (residual.stride(1) == 1 or h == 1)),
-          "rms_norm_mx: residual must have x's shape and dtype and unit column stride")
-    _need(eps >= 0, "rms_norm_mx: eps must not be negative")
-    codes = _mx_codes_like(x, m, h, "mxfp8")
-    scales = torch.empty((mx_scales_numel(m, h, "mxfp8"),), dtype=torch.uint8, device=dev)
-    total = torch.empty((0,) if residual is None else (m, h), dtype=x.dtype, device=dev)
-    if m == 0:
-        return codes, scales, total
-    with _on(dev):
-        _lib.call("svdq_rms_norm_mx", x.data_ptr(), _ld(x), _p(residual), 0 if residual is None else _ld(residual),
-                  _p(weight), _DT[x.dtype], eps, m, h, codes.data_ptr(), scales.data_ptr(), _p(total), h,
-                  _raw_stream(dev))
+    dev = _mx_device("rms_norm_mx", x, weight, residual)
+    m, h, ld = _mx_rows("rms_norm_mx", x)
+    if weight is not None and (weight.dtype != x.dtype or weight.dim() != 1 or weight.shape[0] != h
+                               or not weight.is_contiguous()):
+        raise ValueError(f"rms_norm_mx: weight must be contiguous {x.dtype} [{h}]")
+    if not eps >= 0:
+        raise ValueError("rms_norm_mx: eps must not be negative")
+    ldr = 0
+    if residual is not None:
+        if residual.dtype != x.dtype or residual.shape != x.shape:
+            raise ValueError("rms_norm_mx: residual must have x's shape and dtype")
+        _, _, ldr = _mx_rows("rms_norm_mx (residual)", residual)
+    codes = x.new_empty((m, mx_k_pad(h)), dtype=torch.float8_e4m3fn)
+    scales = x.new_empty((mx_scales_numel(m, h, "mxfp8"),), dtype=torch.uint8)
+    total = x.new_empty((0,) if residual is None else (m, h))
+    if m:
+        with _on(dev):
+            _lib.call("svdq_rms_norm_mx", x.data_ptr(), ld, _ptr(residual), ldr, _ptr(weight), _DT[x.dtype], eps, m, h,
+                      codes.data_ptr(), scales.data_ptr(), None if residual is None else total.data_ptr(), h,
+                      _raw_stream(dev))
     return codes, scales, total
 
 
