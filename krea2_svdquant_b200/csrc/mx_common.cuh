@@ -72,68 +72,90 @@ __device__ __forceinline__ float mx_inverse_scale(uint32_t byte) {
   return byte == 255 ? 0.0f : __uint_as_float((254u - byte) << 23);
 }
 
-// nvfp4 scale byte: e4m3(amax / (6 g)), correctly rounded.  The quotient is taken in 64 bits, where
-// a value that is not halfway between two e4m3 values stays off it, and reaches 32 bits rounded to
-// odd (truncated, with the last bit set when anything was cut off), which keeps it off too.
-// NaN (0x7F) where amax or the quotient is not finite or the tensor scale is not positive.
-__device__ __forceinline__ uint32_t nvfp4_scale_byte(uint32_t amax_bits, float g) {
-  const double t = (double)__uint_as_float(amax_bits) / (6.0 * (double)g);
-  if (amax_bits >= 0x7F800000u || !(t >= 0.0) || !(g > 0.0f && g <= 3.402823466e38f)) return 0x7Fu;
-  const float f = __double2float_rz(t);
-  const float odd = (double)f == t ? f : __uint_as_float(__float_as_uint(f) | 1u);
-  return e4m3x2_satfinite(odd, 0.0f) & 0xFFu;
+// The correctly rounded quotient q = x / h, moved to odd: where x / (h + l) is not exactly q, the
+// neighbour of q on its side, or q itself, whose last bit is set.  Rounding that to a type with at
+// least two bits fewer gives the rounding of the exact quotient.
+__device__ __forceinline__ float to_odd(float q, float x, float h, float l) {
+  const float r = fmaf(-q, l, fmaf(-q, h, x));  // x - q (h + l): the inner difference is exact
+  const uint32_t u = __float_as_uint(q);
+  const int side = ((int)(__float_as_uint(r) ^ u) >> 31) | 1;  // the exact quotient is larger (1) or smaller (-1)
+  return r != 0.0f && (u & 1u) == 0u ? __uint_as_float(u + (uint32_t)side) : q;
 }
-// e2m1 code of q, ties to even, from comparisons (the rare path below).
+// x / h, correctly rounded, from y = the rounded reciprocal of h (P. Markstein, IBM J. R&D 34(1), 1990),
+// while neither h, x nor the quotient is near the ends of fp32's range.
+__device__ __forceinline__ float quotient(float x, float h, float y) {
+  const float q = x * y;
+  return fmaf(fmaf(-q, h, x), y, q);
+}
+
+// nvfp4 scale byte: e4m3(amax / (6 g)) of the exact quotient, through a quotient rounded to odd (in 64
+// bits at the ends of the range).  NaN (0x7F) where amax is not finite or the tensor scale is not a
+// positive number.
+__device__ __forceinline__ uint32_t nvfp4_scale_byte(uint32_t amax_bits, float g) {
+  const float amax = __uint_as_float(amax_bits);
+  const float h = 6.0f * g, l = fmaf(6.0f, g, -h);
+  float t;
+  if (h >= 1.0e-25f && h <= 1.0e25f && amax <= h * 65536.0f) {
+    t = to_odd(quotient(amax, h, __frcp_rn(h)), amax, h, l);
+  } else {
+    const double d = (double)amax / (6.0 * (double)g);
+    if (!(amax_bits < 0x7F800000u && g > 0.0f && __float_as_uint(g) < 0x7F800000u)) return 0x7Fu;
+    t = __double2float_rz(d);
+    if ((double)t != d) t = __uint_as_float(__float_as_uint(t) | 1u);
+  }
+  return e4m3x2_satfinite(t, 0.0f) & 0xFFu;
+}
+// e2m1 code of q, ties to even, from comparisons.
 __device__ __forceinline__ uint32_t e2m1_of(double q) {
   const double a = fabs(q);
   const uint32_t c = (a > 0.25) + (a >= 0.75) + (a > 1.25) + (a >= 1.75) + (a > 2.5) + (a >= 3.5) + (a > 5.0);
   return c | (signbit(q) ? 8u : 0u);
 }
-// 16 values of an nvfp4 block as codes e2m1(x / (sf g)) of the exact quotient.  d = fl32(sf g) and
-// x / d is formed correctly rounded from the reciprocal (Markstein's correction, P. Markstein, IBM
-// J. R&D 34(1), 1990).  That decides every code unless the rounded quotient lands on a border
-// between two codes without being there: impossible when sf g has at most 16 significant bits and
-// x at most 11 (x - border * d is then zero or above 2^-19 of x); otherwise such blocks are redone
-// in 64 bits, as are blocks whose d or quotients leave the range the correction needs.
+// An nvfp4 block whose scale or values are near the ends of fp32's range, in 64 bits.
+static __device__ __noinline__ uint2 nvfp4_codes_wide(const float* x, float sf, float g) {
+  const double d = (double)sf * (double)g;
+  uint32_t w[2] = {0u, 0u};
+#pragma unroll 1
+  for (int i = 0; i < 16; ++i) w[i >> 3] |= e2m1_of((double)x[i] / d) << (4 * (i & 7));
+  return make_uint2(w[0], w[1]);
+}
+// 16 values of an nvfp4 block as codes e2m1(x / (sf g)) of the exact quotient.  d = fl32(sf g) and x / d
+// is formed correctly rounded.  That decides every code unless the rounded quotient lands on a
+// border between two codes without being there: impossible when d = sf g has at most 16
+// significant bits and x at most 11 (x - border * d is then zero or above 2^-19 of x).  Otherwise a
+// block with a quotient of at most 3 significant bits, as borders are, moves its quotients to odd.
+// Takes -x: with q0 = (-x)(-y), r = q0 d - x and q = q0 - r y a zero keeps its sign.
 template <bool SHORT_X>
-__device__ __forceinline__ uint2 nvfp4_codes(const float (&x)[16], uint32_t amax_bits, uint32_t sf_byte, float g) {
+__device__ __forceinline__ uint2 nvfp4_codes(const float (&nx)[16], uint32_t amax_bits, uint32_t sf_byte, float g) {
   const float sf = e4m3_value(sf_byte);
   if (sf_byte == 0u || sf_byte == 0x7Fu) return make_uint2(0u, 0u);
   const float d = sf * g;
   const float dl = fmaf(sf, g, -d);
-  bool redo = !(d >= 8.0e-28f && d <= 1.0e30f && __uint_as_float(amax_bits) <= d * 65536.0f);
+  if (!(d >= 8.0e-28f && d <= 1.0e30f && __uint_as_float(amax_bits) <= d * 65536.0f)) {
+    float v[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = -nx[i];
+    return nvfp4_codes_wide(v, sf, g);
+  }
   const float y = __frcp_rn(d);
+  const uint64_t ny = f2_pack(-y, -y), dd = f2_pack(d, d);
   float q[16];
 #pragma unroll
   for (int i = 0; i < 16; i += 2) {
-    const uint64_t xx = f2_pack(x[i], x[i + 1]);
-    const uint64_t yy = f2_pack(y, y), nd = f2_pack(-d, -d);
-    const uint64_t q0 = f2_mul(xx, yy);
-    const uint64_t qq = f2_fma(f2_fma(q0, nd, xx), yy, q0);
+    const uint64_t xx = f2_pack(nx[i], nx[i + 1]);
+    const uint64_t q0 = f2_mul(xx, ny);
+    const uint64_t qq = f2_fma(f2_fma(q0, dd, xx), ny, q0);
     q[i] = f2_lo(qq);
     q[i + 1] = f2_hi(qq);
   }
   if (!SHORT_X || dl != 0.0f || (__float_as_uint(d) & 0xFFu) != 0u) {
+    bool near_border = false;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) redo |= (__float_as_uint(q[i]) << 11) == 0u && q[i] != 0.0f;
-  }
-  if (redo) {
-    const double dd = (double)sf * (double)g;
-    uint2 w = make_uint2(0u, 0u);
-#pragma unroll 1
-    for (int i = 0; i < 8; ++i) {
-      float a = 0.f, b = 0.f;
+    for (int i = 0; i < 16; ++i) near_border |= (__float_as_uint(q[i]) & 0x1FFFFFu) == 0u;
+    if (near_border) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (j == i) {
-          a = x[j];
-          b = x[8 + j];
-        }
-      }
-      w.x |= e2m1_of((double)a / dd) << (4 * i);
-      w.y |= e2m1_of((double)b / dd) << (4 * i);
+      for (int i = 0; i < 16; ++i) q[i] = to_odd(q[i], -nx[i], d, dl);
     }
-    return w;
   }
   return make_uint2(e2m1x8_satfinite(q), e2m1x8_satfinite(q + 8));
 }
@@ -155,37 +177,88 @@ __device__ __forceinline__ __half from_float<__half>(float v) { return __float2h
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// N values of a row from column c: 16-byte loads where the row allows them and all N columns
-// exist, element by element up to K otherwise (zero past it).
-template <typename T, int N>
-__device__ __forceinline__ void load_cols(const T* row, int c, int K, bool vec, T (&v)[N]) {
-  if (vec && c + N <= K) {
-    constexpr int W = N * (int)sizeof(T) / 16;
-    const uint4* p = reinterpret_cast<const uint4*>(row + c);
+// Bits of the largest magnitude of N values; a NaN is larger than every number.
+template <int N>
+__device__ __forceinline__ uint32_t amax_bits_of(const float (&v)[N]) {
+  float m = 0.0f;
 #pragma unroll
-    for (int i = 0; i < W; ++i) reinterpret_cast<uint4*>(v)[i] = p[i];
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = c + i < K ? row[c + i] : from_float<T>(0.0f);
-  }
-}
-template <typename T, int N>
-__device__ __forceinline__ void store_cols(T* row, int c, int K, bool vec, const T (&v)[N]) {
-  if (vec && c + N <= K) {
-    constexpr int W = N * (int)sizeof(T) / 16;
-    uint4* p = reinterpret_cast<uint4*>(row + c);
-#pragma unroll
-    for (int i = 0; i < W; ++i) p[i] = reinterpret_cast<const uint4*>(v)[i];
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (c + i < K) row[c + i] = v[i];
-  }
+  for (int i = 0; i < N; ++i) asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(m), "f"(fabsf(v[i])));
+  return __float_as_uint(m);
 }
 
-// Rows of a matrix start on 16-byte boundaries.
-inline bool rows_aligned16(const void* p, int64_t ld, int elem_bytes) {
-  return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && (ld * elem_bytes) % 16 == 0;
+// N values of a row from column c (N elements are 16, 32 or 64 bytes) where all of them exist and the
+// row is aligned to them (up to 32 bytes).
+template <typename T, int N>
+__device__ __forceinline__ void load_vec(const T* p, T (&v)[N]) {
+  constexpr int kBytes = N * (int)sizeof(T);
+  if constexpr (kBytes % 32 == 0) {
+#pragma unroll
+    for (int i = 0; i < kBytes / 32; ++i) {
+      uint32_t* w = reinterpret_cast<uint32_t*>(v) + 8 * i;
+      asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                   : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                   : "l"(reinterpret_cast<const uint8_t*>(p) + 32 * i)
+                   : "memory");
+    }
+  } else {
+    *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(p);
+  }
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_vec(T* p, const T (&v)[N]) {
+  constexpr int kBytes = N * (int)sizeof(T);
+  if constexpr (kBytes % 32 == 0) {
+#pragma unroll
+    for (int i = 0; i < kBytes / 32; ++i) {
+      const uint32_t* w = reinterpret_cast<const uint32_t*>(v) + 8 * i;
+      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(reinterpret_cast<uint8_t*>(p) + 32 * i),
+                   "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                   : "memory");
+    }
+  } else {
+    *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(v);
+  }
+}
+// The same for rows that are not aligned or end inside: lane l of the warp owns columns c .. c + N - 1
+// of the row at `row`, and the warp goes over all of its elements 32 at a time, neighbouring lanes at
+// neighbouring columns, through `stage` (32 N elements of shared memory of this warp, 16-byte
+// aligned).  Columns from K on read as zero and are not written.  Every lane takes part.
+template <typename T, int N>
+__device__ __forceinline__ void load_warp(const T* row, int c, int K, T* stage, T (&v)[N]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const int e = j * 32 + lane;
+    const T* p = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(row), e / N));
+    const int col = __shfl_sync(0xffffffffu, c, e / N) + e % N;
+    stage[e] = col < K ? p[col] : from_float<T>(0.0f);
+  }
+  __syncwarp();
+  constexpr int W = N * (int)sizeof(T) / 16;
+#pragma unroll
+  for (int i = 0; i < W; ++i) reinterpret_cast<uint4*>(v)[i] = reinterpret_cast<const uint4*>(stage + lane * N)[i];
+  __syncwarp();
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_warp(T* row, int c, int K, T* stage, const T (&v)[N]) {
+  const int lane = threadIdx.x & 31;
+  constexpr int W = N * (int)sizeof(T) / 16;
+#pragma unroll
+  for (int i = 0; i < W; ++i) reinterpret_cast<uint4*>(stage + lane * N)[i] = reinterpret_cast<const uint4*>(v)[i];
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const int e = j * 32 + lane;
+    T* p = reinterpret_cast<T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(row), e / N));
+    const int col = __shfl_sync(0xffffffffu, c, e / N) + e % N;
+    if (col < K) p[col] = stage[e];
+  }
+  __syncwarp();
+}
+
+// Rows of a matrix start on boundaries of `align` bytes.
+inline bool rows_aligned(const void* p, int64_t ld, int elem_bytes, int align) {
+  return reinterpret_cast<uintptr_t>(p) % align == 0 && (ld * elem_bytes) % align == 0;
 }
 inline int dtype_bytes(int dtype) { return dtype == SVDQ_FP32 ? 4 : 2; }
 inline bool dtype_ok(int dtype) { return dtype == SVDQ_BF16 || dtype == SVDQ_FP16 || dtype == SVDQ_FP32; }

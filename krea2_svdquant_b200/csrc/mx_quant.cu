@@ -22,6 +22,18 @@ __device__ __forceinline__ uint32_t div_by(const FastDiv& f, uint32_t n) {
   return f.d == 1 ? n : __umulhi(n, f.mul) >> (f.shift - 1);
 }
 
+// Chunks of 16 elements per thread: 64 bytes in flight.
+template <typename T>
+__host__ __device__ constexpr int unroll_of() { return sizeof(T) == 2 ? 2 : 1; }
+template <int FMT>
+struct CodeWord {
+  using type = uint2;  // 16 codes
+};
+template <>
+struct CodeWord<kMxfp8> {
+  using type = uint4;
+};
+
 struct QuantArgs {
   const void* x;
   int64_t ldx;
@@ -40,47 +52,39 @@ struct QuantArgs {
 // bf16 to nvfp4.  The four scale bytes of a 32-bit word of the tile layout come from 4 (nvfp4) or 8
 // (mx) neighbouring lanes and leave as one store.
 template <typename T, int FMT>
-__global__ void __launch_bounds__(kThreads) mx_quantize_kernel(const QuantArgs a) {
-  pdl_wait();
-  pdl_trigger();
-  const uint32_t id = blockIdx.x * kThreads + threadIdx.x;
+__device__ __forceinline__ void quantize_chunk(const QuantArgs& a, T (&x)[16], uint32_t id, int row, int chunk,
+                                               bool live, float g) {
   const int lane = threadIdx.x & 31;
-  const uint32_t row_u = div_by(a.per_row, id);
-  const int row = (int)row_u, chunk = (int)(id - row_u * a.per_row.d);
-  const bool live = id < a.chunks && row < a.M;
-  float v[16];
-  uint32_t amax = 0;
-  {
-    T x[16];
-    if (live) {
-      load_cols<T, 16>(static_cast<const T*>(a.x) + (size_t)row * a.ldx, chunk * 16, a.K, a.vec, x);
-    } else {
+  if constexpr (FMT == kNvfp4) {  // nvfp4_codes takes -x
+    constexpr uint32_t kSigns = sizeof(T) == 2 ? 0x80008000u : 0x80000000u;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] = from_float<T>(0.0f);
-    }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      v[i] = to_float(x[i]);
-      amax = max(amax, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-    }
+    for (int i = 0; i < (int)sizeof(T) * 4; ++i) reinterpret_cast<uint32_t*>(x)[i] ^= kSigns;
   }
+  float v[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = to_float(x[i]);
+  uint32_t amax = amax_bits_of(v);
   if (FMT != kNvfp4) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
   uint32_t byte = 0;
   if (live) {
     const size_t code_row = (size_t)row * mx_row_bytes(FMT, (int)a.per_row.d * 16);
     if constexpr (FMT == kNvfp4) {
-      const float g = a.tensor_scale ? *a.tensor_scale : 1.0f;
       byte = nvfp4_scale_byte(amax, g);
       *reinterpret_cast<uint2*>(a.codes + code_row + chunk * 8) = nvfp4_codes<sizeof(T) == 2>(v, amax, byte, g);
     } else {
       byte = mx_scale_byte<FMT>(amax);
       const float inv = mx_inverse_scale(byte);
+      const uint64_t ii = f2_pack(inv, inv);
+#pragma unroll
+      for (int i = 0; i < 16; i += 2) {
+        const uint64_t p = f2_mul(f2_pack(v[i], v[i + 1]), ii);
+        v[i] = f2_lo(p);
+        v[i + 1] = f2_hi(p);
+      }
       if (byte == 255u) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) v[i] = 0.0f;
       }
-#pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] *= inv;
       if constexpr (FMT == kMxfp4) {
         *reinterpret_cast<uint2*>(a.codes + code_row + chunk * 8) =
             make_uint2(e2m1x8_satfinite(v), e2m1x8_satfinite(v + 8));
@@ -102,6 +106,42 @@ __global__ void __launch_bounds__(kThreads) mx_quantize_kernel(const QuantArgs a
         word;
 }
 
+// A CTA takes kThreads * kUnroll neighbouring chunks and issues all its loads first.  VEC: rows on
+// 32-byte boundaries and K a multiple of 16.
+template <typename T, int FMT, bool VEC>
+__global__ void __launch_bounds__(kThreads) mx_quantize_kernel(const QuantArgs a) {
+  constexpr int kUnroll = unroll_of<T>();
+  __shared__ __align__(16) T stage[VEC ? 1 : kThreads * 16];
+  pdl_wait();
+  pdl_trigger();
+  const float g = a.tensor_scale ? *a.tensor_scale : 1.0f;
+  alignas(32) T x[kUnroll][16];
+  uint32_t id[kUnroll];
+  int row[kUnroll], chunk[kUnroll];
+  bool live[kUnroll];
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    id[u] = (blockIdx.x * kUnroll + u) * kThreads + threadIdx.x;
+    const uint32_t r = div_by(a.per_row, id[u]);
+    row[u] = (int)r;
+    chunk[u] = (int)(id[u] - r * a.per_row.d);
+    live[u] = id[u] < a.chunks && row[u] < a.M;
+    const T* src = static_cast<const T*>(a.x) + (live[u] ? (size_t)row[u] * a.ldx : 0);
+    if constexpr (VEC) {
+      if (live[u] && chunk[u] * 16 < a.K) {
+        load_vec(src + chunk[u] * 16, x[u]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[u][i] = from_float<T>(0.0f);
+      }
+    } else {
+      load_warp(src, live[u] ? chunk[u] * 16 : a.K, a.K, stage + (threadIdx.x & ~31) * 16, x[u]);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) quantize_chunk<T, FMT>(a, x[u], id[u], row[u], chunk[u], live[u], g);
+}
+
 struct ReadArgs {
   const uint8_t* codes;
   const uint8_t* scales;
@@ -116,50 +156,60 @@ struct ReadArgs {
 
 // Reading back: one thread turns 16 codes into values, code * scale (* tensor scale) in fp32,
 // rounded once to T.  Bound by HBM (0.56 bytes read, 2 written per element from nvfp4 to bf16).
-template <typename T, int FMT>
+template <typename T, int FMT, bool VEC>
 __global__ void __launch_bounds__(kThreads) mx_dequantize_kernel(const ReadArgs a) {
+  constexpr int kUnroll = unroll_of<T>();
+  __shared__ __align__(16) T stage[VEC ? 1 : kThreads * 16];
   pdl_wait();
   pdl_trigger();
-  const uint32_t id = blockIdx.x * kThreads + threadIdx.x;
-  if (id >= a.chunks) return;
-  const uint32_t row_u = div_by(a.per_row, id);
-  const int row = (int)row_u, chunk = (int)(id - row_u * a.per_row.d);
   const int blocks = (int)a.per_row.d * 16 / mx_block(FMT);
-  const int block = chunk * 16 / mx_block(FMT);
-  const uint32_t byte = a.scales[mx_scale_word(row, block >> 2, blocks >> 2) + (block & 3)];
-  float unit;
-  if constexpr (FMT == kNvfp4)
-    unit = e4m3_value(byte) * (a.tensor_scale ? *a.tensor_scale : 1.0f);
-  else
-    unit = e8m0_value(byte);
-  const uint8_t* src = a.codes + (size_t)row * mx_row_bytes(FMT, (int)a.per_row.d * 16);
-  T v[16];
-  if constexpr (FMT == kMxfp8) {
-    const uint4 w = *reinterpret_cast<const uint4*>(src + chunk * 16);
-    const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+  const float g = FMT == kNvfp4 && a.tensor_scale ? *a.tensor_scale : 1.0f;
+  using Codes = typename CodeWord<FMT>::type;
+  Codes w[kUnroll];
+  uint32_t byte[kUnroll];
+  int row[kUnroll], chunk[kUnroll];
+  bool live[kUnroll];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      uint32_t h2;
-      asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"((uint16_t)(ww[i >> 1] >> (16 * (i & 1)))));
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h2));
-      v[2 * i] = from_float<T>(f.x * unit);
-      v[2 * i + 1] = from_float<T>(f.y * unit);
-    }
-  } else {
-    const uint2 w = *reinterpret_cast<const uint2*>(src + chunk * 8);
-    const uint32_t ww[2] = {w.x, w.y};
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      uint32_t h2;
-      asm("{\n\t.reg .b8 b, c;\n\tmov.b16 {b, c}, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, b;\n\t}"
-          : "=r"(h2)
-          : "h"((uint16_t)((ww[i >> 2] >> (8 * (i & 3))) & 0xFFu)));
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h2));
-      v[2 * i] = from_float<T>(f.x * unit);
-      v[2 * i + 1] = from_float<T>(f.y * unit);
+  for (int u = 0; u < kUnroll; ++u) {
+    const uint32_t id = (blockIdx.x * kUnroll + u) * kThreads + threadIdx.x;
+    const uint32_t r = div_by(a.per_row, id);
+    row[u] = (int)r;
+    chunk[u] = (int)(id - r * a.per_row.d);
+    live[u] = id < a.chunks && chunk[u] * 16 < a.K;
+    w[u] = Codes{};
+    byte[u] = 0;
+    if (live[u]) {
+      const int block = chunk[u] * 16 / mx_block(FMT);
+      byte[u] = a.scales[mx_scale_word(row[u], block >> 2, blocks >> 2) + (block & 3)];
+      w[u] = reinterpret_cast<const Codes*>(a.codes + (size_t)row[u] * mx_row_bytes(FMT, (int)a.per_row.d * 16))[chunk[u]];
     }
   }
-  store_cols<T, 16>(static_cast<T*>(a.out) + (size_t)row * a.ldo, chunk * 16, a.K, a.vec, v);
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    const float unit = FMT == kNvfp4 ? e4m3_value(byte[u]) * g : e8m0_value(byte[u]);
+    const uint32_t* ww = reinterpret_cast<const uint32_t*>(&w[u]);
+    alignas(32) T v[16];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      uint32_t h2;
+      if constexpr (FMT == kMxfp8) {
+        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"((uint16_t)(ww[i >> 1] >> (16 * (i & 1)))));
+      } else {  // the conversion takes the low byte; with other bits above it, it gave wrong values
+        asm("{\n\t.reg .b8 b, c;\n\tmov.b16 {b, c}, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, b;\n\t}"
+            : "=r"(h2)
+            : "h"((uint16_t)((ww[i >> 2] >> (8 * (i & 3))) & 0xFFu)));
+      }
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h2));
+      v[2 * i] = from_float<T>(f.x * unit);
+      v[2 * i + 1] = from_float<T>(f.y * unit);
+    }
+    T* dst = static_cast<T*>(a.out) + (live[u] ? (size_t)row[u] * a.ldo : 0);
+    if constexpr (VEC) {
+      if (live[u]) store_vec(dst + chunk[u] * 16, v);
+    } else {
+      store_warp(dst, live[u] ? chunk[u] * 16 : a.K, a.K, stage + (threadIdx.x & ~31) * 16, v);
+    }
+  }
 }
 
 // Largest magnitude of a matrix as fp32 bits, by an integer maximum: any order gives the same
@@ -170,10 +220,19 @@ __global__ void __launch_bounds__(kThreads) mx_amax_kernel(const T* x, int64_t l
   uint32_t amax = 0;
   for (uint64_t i = (uint64_t)blockIdx.x * kThreads + threadIdx.x; i < chunks; i += (uint64_t)gridDim.x * kThreads) {
     const uint32_t row = div_by(per_row, (uint32_t)i);
-    T v[16];
-    load_cols<T, 16>(x + (size_t)row * ldx, (int)((uint32_t)i - row * per_row.d) * 16, K, vec, v);
+    const int c = (int)((uint32_t)i - row * per_row.d) * 16;
+    if (vec) {
+      if (c >= K) continue;
+      alignas(32) T v[16];
+      float f[16];
+      load_vec(x + (size_t)row * ldx + c, v);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) amax = max(amax, __float_as_uint(to_float(v[j])) & 0x7FFFFFFFu);
+      for (int j = 0; j < 16; ++j) f[j] = to_float(v[j]);
+      amax = max(amax, amax_bits_of(f));
+    } else {
+      for (int j = c; j < c + 16 && j < K; ++j)
+        amax = max(amax, __float_as_uint(to_float(x[(size_t)row * ldx + j])) & 0x7FFFFFFFu);
+    }
   }
   amax = __reduce_max_sync(0xffffffffu, amax);
   if ((threadIdx.x & 31) == 0) atomicMax(out, amax);
@@ -194,21 +253,23 @@ bool chunk_grid(int rows, int K, uint32_t* chunks, FastDiv* per_row) {
   return true;
 }
 
-template <typename T>
+template <typename T, bool VEC>
 int launch_quantize(int fmt, const QuantArgs& a, cudaStream_t stream) {
-  const dim3 grid((a.chunks + kThreads - 1) / kThreads);
+  const uint32_t per = kThreads * unroll_of<T>();
+  const dim3 grid((a.chunks + per - 1) / per), block(kThreads);
   const char* what = "svdq_mx_quantize launch";
-  if (fmt == kNvfp4) return launch_pdl(what, mx_quantize_kernel<T, kNvfp4>, grid, dim3(kThreads), 0, stream, 1, a);
-  if (fmt == kMxfp4) return launch_pdl(what, mx_quantize_kernel<T, kMxfp4>, grid, dim3(kThreads), 0, stream, 1, a);
-  return launch_pdl(what, mx_quantize_kernel<T, kMxfp8>, grid, dim3(kThreads), 0, stream, 1, a);
+  if (fmt == kNvfp4) return launch_pdl(what, mx_quantize_kernel<T, kNvfp4, VEC>, grid, block, 0, stream, 1, a);
+  if (fmt == kMxfp4) return launch_pdl(what, mx_quantize_kernel<T, kMxfp4, VEC>, grid, block, 0, stream, 1, a);
+  return launch_pdl(what, mx_quantize_kernel<T, kMxfp8, VEC>, grid, block, 0, stream, 1, a);
 }
-template <typename T>
+template <typename T, bool VEC>
 int launch_dequantize(int fmt, const ReadArgs& a, cudaStream_t stream) {
-  const dim3 grid((a.chunks + kThreads - 1) / kThreads);
+  const uint32_t per = kThreads * unroll_of<T>();
+  const dim3 grid((a.chunks + per - 1) / per), block(kThreads);
   const char* what = "svdq_mx_dequantize launch";
-  if (fmt == kNvfp4) return launch_pdl(what, mx_dequantize_kernel<T, kNvfp4>, grid, dim3(kThreads), 0, stream, 1, a);
-  if (fmt == kMxfp4) return launch_pdl(what, mx_dequantize_kernel<T, kMxfp4>, grid, dim3(kThreads), 0, stream, 1, a);
-  return launch_pdl(what, mx_dequantize_kernel<T, kMxfp8>, grid, dim3(kThreads), 0, stream, 1, a);
+  if (fmt == kNvfp4) return launch_pdl(what, mx_dequantize_kernel<T, kNvfp4, VEC>, grid, block, 0, stream, 1, a);
+  if (fmt == kMxfp4) return launch_pdl(what, mx_dequantize_kernel<T, kMxfp4, VEC>, grid, block, 0, stream, 1, a);
+  return launch_pdl(what, mx_dequantize_kernel<T, kMxfp8, VEC>, grid, block, 0, stream, 1, a);
 }
 
 }  // namespace
@@ -239,13 +300,13 @@ extern "C" int svdq_mx_quantize(const void* x, int64_t ldx, int dtype, int M, in
   a.M = M;
   a.K = K;
   a.rows = mx_rows_pad(M);
-  a.vec = rows_aligned16(x, ldx, dtype_bytes(dtype));
+  a.vec = K % 16 == 0 && rows_aligned(x, ldx, dtype_bytes(dtype), 32);
   a.tensor_scale = tensor_scale;
   a.codes = static_cast<uint8_t*>(codes);
   a.scales = static_cast<uint8_t*>(scales);
-  if (dtype == SVDQ_BF16) return launch_quantize<__nv_bfloat16>(format, a, stream);
-  if (dtype == SVDQ_FP16) return launch_quantize<__half>(format, a, stream);
-  return launch_quantize<float>(format, a, stream);
+  if (dtype == SVDQ_BF16) return a.vec ? launch_quantize<__nv_bfloat16, true>(format, a, stream) : launch_quantize<__nv_bfloat16, false>(format, a, stream);
+  if (dtype == SVDQ_FP16) return a.vec ? launch_quantize<__half, true>(format, a, stream) : launch_quantize<__half, false>(format, a, stream);
+  return a.vec ? launch_quantize<float, true>(format, a, stream) : launch_quantize<float, false>(format, a, stream);
 }
 
 extern "C" int svdq_mx_dequantize(const void* codes, const void* scales, int format, const float* tensor_scale, int M,
@@ -267,12 +328,12 @@ extern "C" int svdq_mx_dequantize(const void* codes, const void* scales, int for
   a.tensor_scale = tensor_scale;
   a.M = M;
   a.K = K;
-  a.vec = rows_aligned16(out, ldo, dtype_bytes(dtype));
+  a.vec = K % 16 == 0 && rows_aligned(out, ldo, dtype_bytes(dtype), 32);
   a.out = out;
   a.ldo = ldo;
-  if (dtype == SVDQ_BF16) return launch_dequantize<__nv_bfloat16>(format, a, stream);
-  if (dtype == SVDQ_FP16) return launch_dequantize<__half>(format, a, stream);
-  return launch_dequantize<float>(format, a, stream);
+  if (dtype == SVDQ_BF16) return a.vec ? launch_dequantize<__nv_bfloat16, true>(format, a, stream) : launch_dequantize<__nv_bfloat16, false>(format, a, stream);
+  if (dtype == SVDQ_FP16) return a.vec ? launch_dequantize<__half, true>(format, a, stream) : launch_dequantize<__half, false>(format, a, stream);
+  return a.vec ? launch_dequantize<float, true>(format, a, stream) : launch_dequantize<float, false>(format, a, stream);
 }
 
 extern "C" int svdq_mx_tensor_scale(const void* x, int64_t ldx, int dtype, int M, int K, float* out,
@@ -288,7 +349,7 @@ extern "C" int svdq_mx_tensor_scale(const void* x, int64_t ldx, int dtype, int M
   if (M > (1 << 30) || K > (1 << 30) || !chunk_grid(M, K, &chunks, &per_row))
     return set_error(SVDQ_ERR_UNSUPPORTED, "svdq_mx_tensor_scale: more than 2^35 padded elements");
   if (chunks > 0) {
-    const bool vec = rows_aligned16(x, ldx, dtype_bytes(dtype));
+    const bool vec = K % 16 == 0 && rows_aligned(x, ldx, dtype_bytes(dtype), 32);
     const uint32_t want = (chunks + kThreads - 1) / kThreads, most = (uint32_t)num_sms() * 8;
     const dim3 grid(want < most ? want : most), block(kThreads);
     uint32_t* bits = reinterpret_cast<uint32_t*>(out);
