@@ -119,26 +119,66 @@ static __device__ __noinline__ uint2 nvfp4_codes_wide(const float* x, float sf, 
   for (int i = 0; i < 16; ++i) w[i >> 3] |= e2m1_of((double)x[i] / d) << (4 * (i & 7));
   return make_uint2(w[0], w[1]);
 }
-// 16 values of an nvfp4 block as codes e2m1(x / (sf g)) of the exact quotient.  d = fl32(sf g) and x / d
-// is formed correctly rounded.  That decides every code unless the rounded quotient lands on a
-// border between two codes without being there: impossible when d = sf g has at most 16
-// significant bits and x at most 11 (x - border * d is then zero or above 2^-19 of x).  Otherwise a
-// block with a quotient of at most 3 significant bits, as borders are, moves its quotients to odd.
-// Takes -x: with q0 = (-x)(-y), r = q0 d - x and q = q0 - r y a zero keeps its sign.
-template <bool SHORT_X>
-__device__ __forceinline__ uint2 nvfp4_codes(const float (&nx)[16], uint32_t amax_bits, uint32_t sf_byte, float g) {
-  const float sf = e4m3_value(sf_byte);
-  if (sf_byte == 0u || sf_byte == 0x7Fu) return make_uint2(0u, 0u);
-  const float d = sf * g;
-  const float dl = fmaf(sf, g, -d);
-  if (!(d >= 8.0e-28f && d <= 1.0e30f && __uint_as_float(amax_bits) <= d * 65536.0f)) {
+// What the quotients of an nvfp4 block need, by its scale byte.  A launch has one tensor scale g, so a
+// CTA works this out once per byte.
+struct Nvfp4Unit {
+  float d;        // the divisor: sf g, or a neighbour of it (below)
+  float ny;       // -1 / d, rounded
+  float limit;    // magnitudes up to this take the fp32 quotient (below 0: none)
+  uint32_t odd;   // quotients on a border have to be checked
+};
+
+// Codes are e2m1(x / (sf g)) of the exact quotient.  The correctly rounded x / fl32(sf g) decides them
+// unless it lands on a border b between two codes that the exact quotient only comes close to.  For x
+// of P significant bits (8 in bf16, 11 in fp16) that takes an x within 2^-22 of b sf g; b's
+// significand is m / 4 with m = 4 .. 7, so one x per m and power of two: x_m, m sf g rounded to P
+// bits.  All x_m 2^k lie on the same side of their borders, so a divisor moved by 2^-20 to that side
+// decides them, and no other x is near enough to a border for that to matter if every other m sf g is
+// 2^-18 from its x_m.  Where that does not hold, and for fp32 (P = 24), quotients that have at most 3
+// significant bits, as borders do, are moved to odd one by one.
+// (Common, not an accident: g = amax / 2688 = amax / (7 * 384) with a short amax brings every 7 sf g
+// next to a short number.)
+template <int P>
+__device__ __forceinline__ Nvfp4Unit nvfp4_unit(uint32_t byte, float g) {
+  const float sf = e4m3_value(byte);
+  const float d = sf * g, dl = fmaf(sf, g, -d);
+  Nvfp4Unit u{d, 0.0f, -1.0f, 0u};
+  if (!(d >= 8.0e-28f && d <= 1.0e30f)) return u;  // 64 bits
+  u.limit = d * 65536.0f;
+  if constexpr (P < 24) {
+    bool up = false, down = false, between = false;
+#pragma unroll
+    for (int m = 4; m <= 7; ++m) {
+      constexpr uint32_t drop = 24 - P;
+      const float xm = __uint_as_float((__float_as_uint((float)m * d) + (1u << (drop - 1))) & ~((1u << drop) - 1u));
+      const float delta = fmaf((float)m, d, -xm) + (float)m * dl;
+      const bool close = fabsf(delta) < xm * 0x1p-22f && delta != 0.0f;
+      up |= close && delta > 0.0f;
+      down |= close && delta < 0.0f;
+      between |= !close && fabsf(delta) < xm * 0x1p-18f;
+    }
+    if ((up && down) || ((up || down) && between)) u.odd = 1u;
+    else if (up) u.d = d * (1.0f + 0x1p-20f);
+    else if (down) u.d = d * (1.0f - 0x1p-20f);
+  } else {
+    u.odd = 1u;
+  }
+  u.ny = -__frcp_rn(u.d);
+  return u;
+}
+
+// 16 values of an nvfp4 block as codes.  Takes -x: with q0 = (-x)(-y), r = q0 d - x and q = q0 - r y a
+// zero keeps its sign.
+__device__ __forceinline__ uint2 nvfp4_codes(const float (&nx)[16], uint32_t amax_bits, uint32_t byte,
+                                             const Nvfp4Unit& u, float g) {
+  if (byte == 0u || byte == 0x7Fu) return make_uint2(0u, 0u);
+  if (!(__uint_as_float(amax_bits) <= u.limit)) {
     float v[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) v[i] = -nx[i];
-    return nvfp4_codes_wide(v, sf, g);
+    return nvfp4_codes_wide(v, e4m3_value(byte), g);
   }
-  const float y = __frcp_rn(d);
-  const uint64_t ny = f2_pack(-y, -y), dd = f2_pack(d, d);
+  const uint64_t ny = f2_pack(u.ny, u.ny), dd = f2_pack(u.d, u.d);
   float q[16];
 #pragma unroll
   for (int i = 0; i < 16; i += 2) {
@@ -148,16 +188,35 @@ __device__ __forceinline__ uint2 nvfp4_codes(const float (&nx)[16], uint32_t ama
     q[i] = f2_lo(qq);
     q[i + 1] = f2_hi(qq);
   }
-  if (!SHORT_X || dl != 0.0f || (__float_as_uint(d) & 0xFFu) != 0u) {
+  if (u.odd) {
     bool near_border = false;
 #pragma unroll
     for (int i = 0; i < 16; ++i) near_border |= (__float_as_uint(q[i]) & 0x1FFFFFu) == 0u;
     if (near_border) {
+      const float dl = fmaf(e4m3_value(byte), g, -u.d);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) q[i] = to_odd(q[i], -nx[i], d, dl);
+      for (int i = 0; i < 16; ++i) q[i] = to_odd(q[i], -nx[i], u.d, dl);
     }
   }
   return make_uint2(e2m1x8_satfinite(q), e2m1x8_satfinite(q + 8));
+}
+
+// Multiplies by a power of two (an mx block's 2^-e), two values an instruction.
+template <int N>
+__device__ __forceinline__ void scale_all(float (&v)[N], float f) {
+  const uint64_t ff = f2_pack(f, f);
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    const uint64_t p = f2_mul(f2_pack(v[i], v[i + 1]), ff);
+    v[i] = f2_lo(p);
+    v[i + 1] = f2_hi(p);
+  }
+}
+template <int N>
+__device__ __forceinline__ void e4m3_words(const float (&v)[N], uint32_t (&w)[N / 4]) {
+#pragma unroll
+  for (int i = 0; i < N / 4; ++i)
+    w[i] = e4m3x2_satfinite(v[4 * i], v[4 * i + 1]) | e4m3x2_satfinite(v[4 * i + 2], v[4 * i + 3]) << 16;
 }
 
 template <typename T>
@@ -177,7 +236,7 @@ __device__ __forceinline__ __half from_float<__half>(float v) { return __float2h
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// Bits of the largest magnitude of N values; a NaN is larger than every number.
+// Bits (fp32) of the largest magnitude of N values; a NaN is larger than every number.
 template <int N>
 __device__ __forceinline__ uint32_t amax_bits_of(const float (&v)[N]) {
   float m = 0.0f;
@@ -185,6 +244,30 @@ __device__ __forceinline__ uint32_t amax_bits_of(const float (&v)[N]) {
   for (int i = 0; i < N; ++i) asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(m), "f"(fabsf(v[i])));
   return __float_as_uint(m);
 }
+template <int N>
+__device__ __forceinline__ uint32_t amax_bits_of(const __nv_bfloat16 (&v)[N]) {
+  const __nv_bfloat162* p = reinterpret_cast<const __nv_bfloat162*>(v);
+  __nv_bfloat162 m = __habs2(p[0]);
+#pragma unroll
+  for (int i = 1; i < N / 2; ++i) m = __hmax2_nan(m, __habs2(p[i]));
+  return __float_as_uint(__bfloat162float(__hmax_nan(m.x, m.y)));
+}
+template <int N>
+__device__ __forceinline__ uint32_t amax_bits_of(const __half (&v)[N]) {
+  const __half2* p = reinterpret_cast<const __half2*>(v);
+  __half2 m = __habs2(p[0]);
+#pragma unroll
+  for (int i = 1; i < N / 2; ++i) m = __hmax2_nan(m, __habs2(p[i]));
+  return __float_as_uint(__half2float(__hmax_nan(__low2half(m), __high2half(m))));
+}
+template <typename T>
+__host__ __device__ constexpr int significant_bits();
+template <>
+constexpr int significant_bits<float>() { return 24; }
+template <>
+constexpr int significant_bits<__half>() { return 11; }
+template <>
+constexpr int significant_bits<__nv_bfloat16>() { return 8; }
 
 // N values of a row from column c (N elements are 16, 32 or 64 bytes) where all of them exist and the
 // row is aligned to them (up to 32 bytes).
@@ -219,26 +302,46 @@ __device__ __forceinline__ void store_vec(T* p, const T (&v)[N]) {
     *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(v);
   }
 }
-// The same for rows that are not aligned or end inside: lane l of the warp owns columns c .. c + N - 1
-// of the row at `row`, and the warp goes over all of its elements 32 at a time, neighbouring lanes at
-// neighbouring columns, through `stage` (32 N elements of shared memory of this warp, 16-byte
-// aligned).  Columns from K on read as zero and are not written.  Every lane takes part.
+// The same for a row of any alignment that may end inside: columns from K on are zero.  Reads the
+// aligned 16-byte words that hold a byte of the row (so never a word that is not partly the row's), one
+// more than aligned columns take, and shifts.  A row's shift is the same for all its columns.
 template <typename T, int N>
-__device__ __forceinline__ void load_warp(const T* row, int c, int K, T* stage, T (&v)[N]) {
-  const int lane = threadIdx.x & 31;
+__device__ __forceinline__ void load_shifted(const T* row, int c, int K, T (&v)[N]) {
+  constexpr int kWords = N * (int)sizeof(T) / 4;
+  const uintptr_t at = reinterpret_cast<uintptr_t>(row + c), end = reinterpret_cast<uintptr_t>(row + K);
+  const uintptr_t first = at & ~(uintptr_t)15;
+  uint32_t w[kWords + 4];
 #pragma unroll
-  for (int j = 0; j < N; ++j) {
-    const int e = j * 32 + lane;
-    const T* p = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(row), e / N));
-    const int col = __shfl_sync(0xffffffffu, c, e / N) + e % N;
-    stage[e] = col < K ? p[col] : from_float<T>(0.0f);
+  for (int i = 0; i <= kWords / 4; ++i) {
+    uint4 q = make_uint4(0u, 0u, 0u, 0u);
+    if (c < K && first + 16 * i < end) q = *reinterpret_cast<const uint4*>(first + 16 * i);
+    w[4 * i] = q.x;
+    w[4 * i + 1] = q.y;
+    w[4 * i + 2] = q.z;
+    w[4 * i + 3] = q.w;
   }
-  __syncwarp();
-  constexpr int W = N * (int)sizeof(T) / 16;
+  const uint32_t shift = (uint32_t)(at & 15);
+  if (shift & 8) {
 #pragma unroll
-  for (int i = 0; i < W; ++i) reinterpret_cast<uint4*>(v)[i] = reinterpret_cast<const uint4*>(stage + lane * N)[i];
-  __syncwarp();
+    for (int i = 0; i < kWords + 2; ++i) w[i] = w[i + 2];
+  }
+  if (shift & 4) {
+#pragma unroll
+    for (int i = 0; i < kWords + 1; ++i) w[i] = w[i + 1];
+  }
+  uint32_t* out = reinterpret_cast<uint32_t*>(v);
+#pragma unroll
+  for (int i = 0; i < kWords; ++i) out[i] = sizeof(T) == 4 ? w[i] : __funnelshift_r(w[i], w[i + 1], 8 * (shift & 2));
+  if (c + N > K) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (c + i >= K) v[i] = from_float<T>(0.0f);
+  }
 }
+// The way back, by a warp whose lane l has columns c .. c + N - 1 of the row at `row`: the warp writes
+// its elements 32 at a time, neighbouring lanes at neighbouring columns, through `stage` (32 N
+// elements of shared memory of this warp, 16-byte aligned).  Columns from K on are not written.
+// Every lane takes part.
 template <typename T, int N>
 __device__ __forceinline__ void store_warp(T* row, int c, int K, T* stage, const T (&v)[N]) {
   const int lane = threadIdx.x & 31;

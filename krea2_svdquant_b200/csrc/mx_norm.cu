@@ -23,15 +23,17 @@ struct NormArgs {
   int64_t lds;
 };
 
-// One CTA per row.  A thread owns 8 columns of each 8 * THREADS; four neighbouring lanes share an
-// mx block.  The row and the weight stay in registers between the two steps (the sum of squares, then
-// the codes) for up to PASSES * 8 * THREADS columns; PASSES == 0 reads them again instead.  Bound by
-// HBM: 6 bytes read or written as bf16 and 1.03 as codes per element with a residual.
+// One CTA per row.  A thread owns C columns of each C * THREADS (C = 16, or 8 in fp32: 32 bytes); the
+// 32 / C neighbouring lanes of an mx block share its scale.  The row stays in registers between the
+// two steps (the sum of squares, then the codes) for up to PASSES * C * THREADS columns; PASSES == 0
+// reads it again instead.  Bound by HBM: 6 bytes read or written as bf16 and 1.03 as codes per
+// element with a residual.
 template <typename T, int THREADS, int PASSES, bool VEC>
 __global__ void __launch_bounds__(THREADS) rms_norm_mx_kernel(const NormArgs a) {
+  constexpr int C = 32 / (int)sizeof(T);
   constexpr int kKeep = PASSES > 0 ? PASSES : 1;
   __shared__ float part[THREADS / 32];
-  __shared__ __align__(16) T stage_all[VEC ? 1 : THREADS * 8];
+  __shared__ __align__(16) T stage[VEC ? 1 : THREADS * C];
   pdl_wait();
   pdl_trigger();
   const int row = blockIdx.x;
@@ -41,62 +43,55 @@ __global__ void __launch_bounds__(THREADS) rms_norm_mx_kernel(const NormArgs a) 
     for (int w = tid; w < words; w += THREADS) *reinterpret_cast<uint32_t*>(a.scales + mx_scale_word(row, w, words)) = 0u;
     return;
   }
-  T* stage = stage_all + (VEC ? 0 : (tid & ~31) * 8);
   const T* xr = static_cast<const T*>(a.x) + (size_t)row * a.ldx;
   const T* rr = a.residual ? static_cast<const T*>(a.residual) + (size_t)row * a.ldr : nullptr;
   T* sr = a.sum ? static_cast<T*>(a.sum) + (size_t)row * a.lds : nullptr;
   const T* weight = static_cast<const T*>(a.weight);
-  const int passes = PASSES > 0 ? PASSES : (a.h_pad + 8 * THREADS - 1) / (8 * THREADS);
-  auto load = [&](const T* p, int c, T (&v)[8]) {
-    if constexpr (VEC) {
-      if (c < a.H) {
-        load_vec(p + c, v);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = from_float<T>(0.0f);
-      }
+  const int passes = PASSES > 0 ? PASSES : (a.h_pad + C * THREADS - 1) / (C * THREADS);
+  auto column = [&](int p) { return (p * THREADS + tid) * C; };
+  auto load = [&](const T* p, int c, T (&v)[C]) {
+    if constexpr (!VEC) {
+      load_shifted(p, c, a.H, v);
+    } else if (c < a.H) {
+      load_vec(p + c, v);
     } else {
-      load_warp(p, c, a.H, stage, v);
+#pragma unroll
+      for (int i = 0; i < C; ++i) v[i] = from_float<T>(0.0f);
     }
   };
-  alignas(32) T keep[kKeep][8];
-  alignas(32) T res[kKeep][8];
-  alignas(32) T wt[kKeep][8];
-  float ss = 0.0f;
-  auto add = [&](int c, T (&h)[8], const T (&r)[8]) {
+  alignas(32) T keep[kKeep][C];
+  alignas(32) T res[kKeep][C];
+  uint64_t ss2 = 0;  // two sums of squares
+  auto add = [&](int c, T (&h)[C], const T (&r)[C]) {
     if (rr) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) h[i] = from_float<T>(to_float(h[i]) + to_float(r[i]));
-      if constexpr (VEC) {
-        if (c < a.H) store_vec(sr + c, h);
-      } else {
-        store_warp(sr, c, a.H, stage, h);
-      }
+      for (int i = 0; i < C; ++i) h[i] = from_float<T>(to_float(h[i]) + to_float(r[i]));
+      if constexpr (!VEC) store_warp(sr, c, a.H, stage + (tid & ~31) * C, h);
+      else if (c < a.H) store_vec(sr + c, h);
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ss = fmaf(to_float(h[i]), to_float(h[i]), ss);
+    for (int i = 0; i < C; i += 2) {
+      const uint64_t v = f2_pack(to_float(h[i]), to_float(h[i + 1]));
+      ss2 = f2_fma(v, v, ss2);
+    }
   };
   if constexpr (PASSES > 0) {  // every load first
 #pragma unroll
-    for (int p = 0; p < PASSES; ++p) load(xr, (p * THREADS + tid) * 8, keep[p]);
+    for (int p = 0; p < PASSES; ++p) load(xr, column(p), keep[p]);
     if (rr) {
 #pragma unroll
-      for (int p = 0; p < PASSES; ++p) load(rr, (p * THREADS + tid) * 8, res[p]);
-    }
-    if (weight) {
-#pragma unroll
-      for (int p = 0; p < PASSES; ++p) load(weight, (p * THREADS + tid) * 8, wt[p]);
+      for (int p = 0; p < PASSES; ++p) load(rr, column(p), res[p]);
     }
 #pragma unroll
-    for (int p = 0; p < PASSES; ++p) add((p * THREADS + tid) * 8, keep[p], res[p]);
+    for (int p = 0; p < PASSES; ++p) add(column(p), keep[p], res[p]);
   } else {
     for (int p = 0; p < passes; ++p) {
-      const int c = (p * THREADS + tid) * 8;
-      load(xr, c, keep[0]);
-      if (rr) load(rr, c, res[0]);
-      add(c, keep[0], res[0]);
+      load(xr, column(p), keep[0]);
+      if (rr) load(rr, column(p), res[0]);
+      add(column(p), keep[0], res[0]);
     }
   }
+  float ss = f2_lo(ss2) + f2_hi(ss2);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
   if (lane == 0) part[tid >> 5] = ss;
@@ -105,59 +100,65 @@ __global__ void __launch_bounds__(THREADS) rms_norm_mx_kernel(const NormArgs a) 
 #pragma unroll
   for (int w = 0; w < THREADS / 32; ++w) ss += part[w];
   const float inv = 1.0f / sqrtf(ss / (float)a.H + a.eps);
-  auto encode = [&](int c, const T (&h)[8], const T (&w)[8]) {
-    float y[8];
+  const uint64_t inv2 = f2_pack(inv, inv);
+  auto encode = [&](int c, const T (&h)[C]) {
+    alignas(32) T w[C];
+    if (weight) load(weight, c, w);
+    float y[C];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = to_float(h[i]) * inv;
-    if (weight) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] *= to_float(w[i]);
+    for (int i = 0; i < C; i += 2) {
+      uint64_t v = f2_mul(f2_pack(to_float(h[i]), to_float(h[i + 1])), inv2);
+      if (weight) v = f2_mul(v, f2_pack(to_float(w[i]), to_float(w[i + 1])));
+      y[i] = f2_lo(v);
+      y[i + 1] = f2_hi(v);
     }
     uint32_t amax = amax_bits_of(y);
     amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+    if (C == 8) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
     const uint32_t byte = mx_scale_byte<kMxfp8>(amax);
-    const float f = mx_inverse_scale(byte);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] *= f;
     if (byte == 255u) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = 0.0f;
+      for (int i = 0; i < C; ++i) y[i] = 0.0f;
     }
-    if (c < a.h_pad)
-      *reinterpret_cast<uint2*>(a.codes + (size_t)row * a.h_pad + c) =
-          make_uint2(e4m3x2_satfinite(y[0], y[1]) | e4m3x2_satfinite(y[2], y[3]) << 16,
-                     e4m3x2_satfinite(y[4], y[5]) | e4m3x2_satfinite(y[6], y[7]) << 16);
-    uint32_t word = byte << (8 * ((lane >> 2) & 3));
-    word |= __shfl_xor_sync(0xffffffffu, word, 4);
-    word |= __shfl_xor_sync(0xffffffffu, word, 8);
-    if (c < a.h_pad && (lane & 15) == 0)
-      *reinterpret_cast<uint32_t*>(a.scales + mx_scale_word(row, c >> 7, words)) = word;
+    scale_all(y, mx_inverse_scale(byte));
+    uint32_t q[C / 4];
+    e4m3_words(y, q);
+    constexpr int L = 32 / C;  // lanes per block
+    uint32_t word = byte << (8 * ((lane / L) & 3));
+    word |= __shfl_xor_sync(0xffffffffu, word, L);
+    word |= __shfl_xor_sync(0xffffffffu, word, 2 * L);
+    if (c < a.h_pad) {
+      uint8_t* to = a.codes + (size_t)row * a.h_pad + c;
+      if constexpr (C == 16) *reinterpret_cast<uint4*>(to) = make_uint4(q[0], q[1], q[2], q[3]);
+      else *reinterpret_cast<uint2*>(to) = make_uint2(q[0], q[1]);
+      if (lane % (4 * L) == 0) *reinterpret_cast<uint32_t*>(a.scales + mx_scale_word(row, c >> 7, words)) = word;
+    }
   };
   if constexpr (PASSES > 0) {
 #pragma unroll
-    for (int p = 0; p < PASSES; ++p) encode((p * THREADS + tid) * 8, keep[p], wt[p]);
+    for (int p = 0; p < PASSES; ++p) encode(column(p), keep[p]);
   } else {
     for (int p = 0; p < passes; ++p) {
-      const int c = (p * THREADS + tid) * 8;
-      if constexpr (!VEC) __syncwarp();  // the sums of this warp's columns, as its lanes stored them
-      load(sr ? sr : xr, c, keep[0]);
-      if (weight) load(weight, c, wt[0]);
-      encode(c, keep[0], wt[0]);
+      if constexpr (!VEC) __syncwarp();
+      load(sr ? sr : xr, column(p), keep[0]);  // the sums as this warp stored them
+      encode(column(p), keep[0]);
     }
   }
 }
 
 template <typename T, bool VEC>
 int launch_norm(const NormArgs& a, cudaStream_t stream) {
+  constexpr int C = 32 / (int)sizeof(T);
   const dim3 grid(mx_rows_pad(a.M));
   const char* what = "svdq_rms_norm_mx launch";
-  if (a.h_pad <= 1024) return launch_pdl(what, rms_norm_mx_kernel<T, 128, 1, VEC>, grid, dim3(128), 0, stream, 1, a);
-  if (a.h_pad <= 2048) return launch_pdl(what, rms_norm_mx_kernel<T, 256, 1, VEC>, grid, dim3(256), 0, stream, 1, a);
-  if (a.h_pad <= 4096) return launch_pdl(what, rms_norm_mx_kernel<T, 256, 2, VEC>, grid, dim3(256), 0, stream, 1, a);
-  if (a.h_pad <= 6144) return launch_pdl(what, rms_norm_mx_kernel<T, 256, 3, VEC>, grid, dim3(256), 0, stream, 1, a);
-  if (a.h_pad <= 8192) return launch_pdl(what, rms_norm_mx_kernel<T, 256, 4, VEC>, grid, dim3(256), 0, stream, 1, a);
-  if (a.h_pad <= 16384) return launch_pdl(what, rms_norm_mx_kernel<T, 512, 4, VEC>, grid, dim3(512), 0, stream, 1, a);
+  const int chunks = a.h_pad / C;
+  if (chunks <= 128) return launch_pdl(what, rms_norm_mx_kernel<T, 128, 1, VEC>, grid, dim3(128), 0, stream, 1, a);
+  if (chunks <= 256) return launch_pdl(what, rms_norm_mx_kernel<T, 128, 2, VEC>, grid, dim3(128), 0, stream, 1, a);
+  if (chunks <= 384) return launch_pdl(what, rms_norm_mx_kernel<T, 128, 3, VEC>, grid, dim3(128), 0, stream, 1, a);
+  if (chunks <= 512) return launch_pdl(what, rms_norm_mx_kernel<T, 256, 2, VEC>, grid, dim3(256), 0, stream, 1, a);
+  if (chunks <= 768) return launch_pdl(what, rms_norm_mx_kernel<T, 256, 3, VEC>, grid, dim3(256), 0, stream, 1, a);
+  if (chunks <= 1024) return launch_pdl(what, rms_norm_mx_kernel<T, 256, 4, VEC>, grid, dim3(256), 0, stream, 1, a);
+  if (chunks <= 2048) return launch_pdl(what, rms_norm_mx_kernel<T, 512, 4, VEC>, grid, dim3(512), 0, stream, 1, a);
   return launch_pdl(what, rms_norm_mx_kernel<T, 512, 0, VEC>, grid, dim3(512), 0, stream, 1, a);
 }
 
@@ -189,8 +190,8 @@ extern "C" int svdq_rms_norm_mx(const void* x, int64_t ldx, const void* residual
   a.M = M;
   a.H = H;
   a.h_pad = mx_k_pad(H);
-  const int al = 8 * eb;
-  const bool vec = H % 8 == 0 && rows_aligned(x, ldx, eb, al) &&
+  const int al = 32;
+  const bool vec = H % (32 / eb) == 0 && rows_aligned(x, ldx, eb, al) &&
                    (!residual || (rows_aligned(residual, ldr, eb, al) && rows_aligned(sum, lds, eb, al))) &&
                    reinterpret_cast<uintptr_t>(weight) % al == 0;
   a.codes = static_cast<uint8_t*>(codes);
