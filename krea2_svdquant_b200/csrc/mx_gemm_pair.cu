@@ -65,6 +65,13 @@ struct PairShape {
   static constexpr size_t kSmem = (size_t)kStages * kStage + sizeof(PairBars) + 1024;
 };
 
+// Arrive on an mbarrier of either CTA after reads of tensor memory (completed, and ordered by a
+// tcgen05 fence).  Release at CTA scope: at cluster scope the arrival waits for this thread's output
+// stores of the tile before to be performed, over 1000 cycles in which the next tile cannot start.
+__device__ __forceinline__ void mbar_arrive_after_tmem(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
 __device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y,
                                                  int z) {
   asm volatile(
@@ -317,7 +324,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         if (c == 0) {
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(free_bar);
+          if (lane == 0) mbar_arrive_after_tmem(free_bar);
         }
         if (c < 3) tmem_ld32(acc + (uint32_t)(((first + 2 * (c + 1)) & 7) * 32), nxt);
         store_chunk(a.o, m0, lane, n0 + ((first + 2 * c) & 7) * 32, cur, alpha, wide, bars->turn[warp - 4]);
