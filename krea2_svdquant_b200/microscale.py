@@ -19,6 +19,8 @@ mxfp8     e4m3    32     power of two per block (activations only)
 * :func:`rms_norm`: residual addition, root-mean-square norm and mxfp8 output in one pass, so that
   the linears which read a block's normed activations share one quantisation.
 
+For inference, like :mod:`.linear`: outputs carry no gradient.
+
 The reference has no counterpart: its weights are INT4 with bf16 group scales
 (src/krea2_svdquant/quant/pack.py:6-70).
 """
@@ -96,16 +98,16 @@ def matmul(a: MicroTensor, w: MicroTensor, bias: torch.Tensor | None = None, *,
     return out if len(a.shape) == 2 else out.reshape(*a.shape[:-1], w.shape[0])
 
 
-def linear(x: torch.Tensor | MicroTensor, w: MicroTensor, bias: torch.Tensor | None = None, *, act: str = "nvfp4",
+def linear(x: torch.Tensor | MicroTensor, w: MicroTensor, bias: torch.Tensor | None = None, *, act: str | None = None,
            act_scale: torch.Tensor | None = None, out_dtype: torch.dtype | None = None) -> torch.Tensor:
-    """``x @ w^T + bias`` with x quantised to format ``act`` on the way (``act_scale``: its calibrated
-    nvfp4 tensor scale).  The output has x's dtype unless ``out_dtype`` says otherwise.  An x that is
+    """``x @ w^T + bias`` with x quantised to format ``act`` on the way (None: the weight's own format;
+    ``act_scale``: its calibrated nvfp4 tensor scale).  The output has x's dtype unless ``out_dtype`` says otherwise.  An x that is
     a :class:`MicroTensor` already goes straight to the product (bf16 output by default)."""
     if isinstance(x, MicroTensor):
         return matmul(x, w, bias, out_dtype=out_dtype or torch.bfloat16)
     if len(w.shape) != 2 or x.dim() < 1 or x.shape[-1] != w.shape[1]:
         raise ValueError(f"linear: activations {tuple(x.shape)} and weight {w.shape} do not match")
-    out = _kernels().mx_linear(_rows(x), act, act_scale, w.codes, w.scales, w.fmt, w.tensor_scale, bias,
+    out = _kernels().mx_linear(_rows(x), act or w.fmt, act_scale, w.codes, w.scales, w.fmt, w.tensor_scale, bias,
                                out_dtype or x.dtype)
     return out if x.dim() == 2 else out.reshape(*x.shape[:-1], w.shape[0])
 
@@ -165,6 +167,14 @@ class MicroscaledLinear(nn.Module):
         fmt = ACTIVATIONS[act]
         packed = quantize(w, fmt, tensor_scale=tensor_scale(w) if fmt == "nvfp4" else None)
         return cls(packed, None if layer.bias is None else layer.bias.detach(), act=act, act_scale=act_scale)
+
+    def _apply(self, fn, recurse=True):
+        # .half() / .to(dtype) casts a model's floating buffers; these have one type each and only move
+        kept = {n: b for n in ("weight_scale", "act_scale", "bias") if (b := self._buffers[n]) is not None}
+        super()._apply(fn, recurse)
+        for n, b in kept.items():
+            self._buffers[n] = b.to(self.codes.device)
+        return self
 
     @property
     def weight(self) -> MicroTensor:

@@ -18,6 +18,9 @@
   modulation and RoPE are left out; every quantized linear has the exact
   shape and module path of the real model (``transformer_blocks.{i}.attn.to_q``
   ...), so the checkpoint, LoRA and offload paths address it unchanged.
+  With block-scaled linears (``random_microscaled``, or ``MicroscaledLinear`` put in place of its
+  layers) a norm's output is quantised once for all layers that read it, and with mxfp8 activations
+  the norm itself does that, together with the residual add before it (``microscale.rms_norm``).
 """
 from __future__ import annotations
 
@@ -32,11 +35,12 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
-from . import ops
+from . import microscale, ops
 from .config import BackendKind
 from .linear import SVDQuantLinear, grouped_forward
 from .load import CONFIG_NAME, TENSORS_NAME, load_svdquant_transformer
 from .lora import load_svdquant_lora_adapters
+from .microscale import MicroscaledLinear, MicroTensor
 from .quant import random_state
 
 
@@ -124,11 +128,12 @@ class _Attention(nn.Module):
         self.to_gate = lin("attn.to_gate")
         self.to_out = nn.ModuleList([lin("attn.to_out.0")])
 
-    def forward(self, h: torch.Tensor, b: int, l: int, residual: torch.Tensor | None = None) -> torch.Tensor:
+    def forward(self, h: torch.Tensor | MicroTensor, b: int, l: int, residual: torch.Tensor | None = None) -> torch.Tensor:
         """``to_out(o * sigmoid(to_gate(h)))``, plus ``residual`` when given."""
         c = self.cfg
         # q / k / v read the same h: one grouped GEMM launch when they are SVDQuant layers
-        q, k, v = grouped_forward([self.to_q, self.to_k, self.to_v], h)
+        qkv = [self.to_q, self.to_k, self.to_v]
+        q, k, v = [lin(h) for lin in qkv] if isinstance(h, MicroTensor) else grouped_forward(qkv, h)
         q = q.view(b, l, c.heads, c.head_dim).transpose(1, 2)
         k = k.view(b, l, c.kv_heads, c.head_dim).transpose(1, 2)
         v = v.view(b, l, c.kv_heads, c.head_dim).transpose(1, 2)
@@ -145,7 +150,7 @@ class _FeedForward(nn.Module):
         self.up = lin("ff.up")
         self.down = lin("ff.down")
 
-    def forward(self, h: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
+    def forward(self, h: torch.Tensor | MicroTensor, residual: torch.Tensor | None = None) -> torch.Tensor:
         """``down(silu(gate(h)) * up(h))``, plus ``residual`` when given."""
         prod = _linear(self.up, h, ("silu_mul", self.gate(h)))
         return _linear(self.down, prod, None if residual is None else ("add", residual))
@@ -161,6 +166,25 @@ def _linear(lin: nn.Module, x: torch.Tensor, epilogue: tuple[str, torch.Tensor] 
     return ops.apply_epilogue(lin(x), epilogue)
 
 
+def _quantized_norm(norm: nn.RMSNorm, x: torch.Tensor, act: str, act_scale: torch.Tensor | None,
+                    residual: torch.Tensor | None = None) -> tuple[MicroTensor, torch.Tensor]:
+    """``(norm(h) in format act, h)`` with ``h = x + residual``: the input of several block-scaled
+    linears, quantised once.  For mxfp8 the add, the norm and the quantisation are one kernel."""
+    if act == "mxfp8":
+        return microscale.rms_norm(x, norm.weight, residual=residual, eps=norm.eps)
+    h = x if residual is None else x + residual
+    return microscale.quantize(norm(h), act, tensor_scale=act_scale), h
+
+
+def _shared_format(layers) -> tuple[str, torch.Tensor | None] | None:
+    """The activation format (and tensor scale) that block-scaled layers have in common, or None."""
+    layers = list(layers)
+    if not all(isinstance(lin, MicroscaledLinear) for lin in layers):
+        return None
+    act, scale = layers[0].act, layers[0].act_scale
+    return (act, scale) if all(lin.act == act and lin.act_scale is scale for lin in layers) else None
+
+
 class Krea2StandInBlock(nn.Module):
     def __init__(self, cfg: Krea2StandInConfig, lin, dtype=torch.bfloat16):
         super().__init__()
@@ -173,6 +197,13 @@ class Krea2StandInBlock(nn.Module):
         # x + attn(norm1(x)), then x + ff(norm2(x)); the residual adds (and the gate products
         # inside attn and ff) run in the epilogues of the linears that produce their operands
         b, l, d = x.shape
+        attn, ff = self.attn, self.ff
+        first = _shared_format((attn.to_q, attn.to_k, attn.to_v, attn.to_gate))
+        second = _shared_format((ff.gate, ff.up))
+        if first and second:
+            h, x2 = _quantized_norm(self.norm1, x.reshape(b * l, d), *first)
+            h, x2 = _quantized_norm(self.norm2, attn(h, b, l), *second, residual=x2)
+            return ff(h, residual=x2).view(b, l, d)
         x = self.attn(self.norm1(x).reshape(b * l, d), b, l, residual=x.reshape(b * l, d)).view(b, l, d)
         return self.ff(self.norm2(x).reshape(b * l, d), residual=x.reshape(b * l, d)).view(b, l, d)
 
@@ -210,6 +241,28 @@ class Krea2StandInTransformer(nn.Module):
 
         torch.manual_seed(seed)
         return cls(cfg, make, dtype)
+
+    @classmethod
+    def random_microscaled(cls, cfg: Krea2StandInConfig, *, act: str = "mxfp8", seed: int = 0,
+                           device: str | torch.device = "cuda",
+                           dtype: torch.dtype = torch.bfloat16) -> "Krea2StandInTransformer":
+        """Every listed linear a random-init block-scaled layer with activations in format ``act``
+        (``mxfp8`` or ``mxfp4`` on an mxfp4 weight, ``nvfp4`` on an nvfp4 weight), on ``device``."""
+        if act not in microscale.ACTIVATIONS:
+            raise ValueError(f"act must be one of {sorted(microscale.ACTIVATIONS)}, got {act!r}")
+        gen = torch.Generator(device=device).manual_seed(seed)
+        shapes = cfg.linear_shapes()
+        fmt = microscale.ACTIVATIONS[act]
+
+        def make(i: int, name: str) -> MicroscaledLinear:
+            n, k = shapes[name]
+            w = torch.randn(n, k, generator=gen, device=device, dtype=dtype).mul_(k ** -0.5)
+            scale = microscale.tensor_scale(w) if fmt == "nvfp4" else None
+            return MicroscaledLinear(microscale.quantize(w, fmt, tensor_scale=scale),
+                                     torch.zeros(n, device=device, dtype=torch.bfloat16), act=act)
+
+        torch.manual_seed(seed)
+        return cls(cfg, make, dtype).to(device)
 
     def forward(self, latents: torch.Tensor, text: torch.Tensor) -> torch.Tensor:
         """``latents`` [B, image_tokens, in_channels], ``text`` [B, text_tokens, hidden] -> [B, image_tokens,

@@ -312,6 +312,102 @@ def test_linear_quantises_on_the_way(act):
     assert M.dequantize(a).shape == x.shape
 
 
+@pytest.mark.parametrize("act", ["mxfp8", "nvfp4", "mxfp4"])
+def test_stand_in_model(act):
+    """The stand-in transformer on block-scaled linears: every layer's output against 64 bits on the
+    operands that it received, and the layers behind a norm share one quantised input."""
+    from krea2_svdquant_b200.transformer import Krea2StandInConfig, Krea2StandInTransformer
+    M = ms()
+    cfg = Krea2StandInConfig(num_layers=2, hidden=256, heads=4, kv_heads=2, head_dim=64, mlp=512, in_channels=32,
+                             image_tokens=60, text_tokens=21)
+    model = Krea2StandInTransformer.random_microscaled(cfg, act=act, seed=3)
+    seen = {}
+    for name, mod in model.named_modules():
+        if isinstance(mod, M.MicroscaledLinear):
+            mod.register_forward_hook(lambda m, a, y, name=name: seen.__setitem__(name, (m, a[0], y)))
+    lat, txt = data(120, 32, torch.bfloat16).view(2, 60, 32), data(42, 256, torch.bfloat16).view(2, 21, 256)
+    out = model(lat, txt)
+    assert out.shape == (2, 60, 32) and torch.isfinite(out).all()
+    assert len(seen) == 16
+    for name, (mod, x, y) in seen.items():
+        a = x if isinstance(x, M.MicroTensor) else M.quantize(x, act)
+        check_product(y, operand_values(a), operand_values(mod.weight), mod.bias, torch.bfloat16)
+    for i in range(2):
+        p = f"transformer_blocks.{i}."
+        shared = [seen[p + n][1] for n in ("attn.to_q", "attn.to_k", "attn.to_v", "attn.to_gate")]
+        assert all(isinstance(s, M.MicroTensor) and s is shared[0] for s in shared)
+        assert seen[p + "ff.gate"][1] is seen[p + "ff.up"][1]
+    assert torch.equal(model(lat, txt), out)
+    no_device_error()
+
+
+def test_layers_move_and_keep_their_types():
+    M = ms()
+    lin = M.MicroscaledLinear.from_linear(torch.nn.Linear(130, 70, device="cuda"), act="nvfp4",
+                                          act_scale=torch.tensor([0.1], device="cuda"))
+    x = data(3, 130)
+    y = lin(x)
+    assert torch.equal(lin.half()(x), y) and lin.weight_scale.dtype == torch.float32 and lin.bias.dtype == torch.bfloat16
+    assert torch.equal(lin.cpu().cuda()(x), y)
+    other = M.MicroscaledLinear.from_linear(torch.nn.Linear(130, 70, device="cuda"), act="nvfp4",
+                                            act_scale=torch.tensor([0.1], device="cuda"))
+    other.load_state_dict(lin.state_dict())
+    assert torch.equal(other(x), y)
+
+
+def test_inputs_of_any_layout():
+    """Transposed, expanded, sliced and higher-dimensional inputs."""
+    M = ms()
+    w = M.quantize(data(40, 96, seed=1), "mxfp4")
+    base = data(96, 50)
+    for x in (base.t(), base[:1].reshape(1, 1, 50).expand(3, 4, 50)[..., :1].expand(3, 4, 96),
+              data(12, 200)[:, 7:103], data(24, 96).view(2, 3, 4, 96), data(10, 96)[::2]):
+        dense = x.reshape(-1, 96).contiguous()
+        want = M.linear(dense, w)
+        assert torch.equal(M.linear(x, w).reshape(want.shape), want)
+        for fmt in FORMATS:
+            a, b = M.quantize(x, fmt), M.quantize(dense, fmt)
+            assert torch.equal(a.codes.view(torch.uint8), b.codes.view(torch.uint8)) and torch.equal(a.scales, b.scales)
+        h, s = M.rms_norm(x, residual=x)
+        h2, s2 = M.rms_norm(dense, residual=dense)
+        assert torch.equal(h.codes.view(torch.uint8), h2.codes.view(torch.uint8)) and torch.equal(s.reshape(s2.shape), s2)
+
+
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+@pytest.mark.parametrize("offset", [1, 2, 3, 5, 8])
+def test_rows_that_start_anywhere(dtype, offset):
+    """Row starts at every alignment that the element type allows, at the end of an allocation too."""
+    M, t = ms(), DTYPES[dtype]
+    m, k = 9, 77
+    flat = data(1, m * 83 + offset, t, seed=offset)[0]
+    x = flat[offset:].view(m, 83)[:, 83 - k:]
+    dense = x.contiguous()
+    for fmt in FORMATS:
+        a, b = M.quantize(x, fmt), M.quantize(dense, fmt)
+        check_quantized(a, x, fmt)
+        assert torch.equal(a.scales, b.scales)
+    w = flat[offset:offset + k]
+    h, s = M.rms_norm(x, w, residual=x)
+    h2, s2 = M.rms_norm(dense, w.clone(), residual=dense)
+    assert torch.equal(h.codes.view(torch.uint8), h2.codes.view(torch.uint8)) and torch.equal(s, s2)
+    assert M.tensor_scale(x).item() == M.tensor_scale(dense).item()
+
+
+def test_norm_in_place_through_the_c_abi():
+    """sum may be x or the residual itself; columns past H of a wider sum stay as they were."""
+    from krea2_svdquant_b200 import _lib, ops
+    for h in (96, 101, 40000):
+        x, r = data(5, h, torch.bfloat16), data(5, h, torch.bfloat16, seed=1)
+        q, total = ms().rms_norm(x, residual=r)
+        wide = torch.full((5, h + 11), 3.0, dtype=torch.bfloat16, device="cuda")
+        wide[:, :h] = r
+        codes, scales = torch.empty_like(q.codes), torch.empty_like(q.scales)
+        _lib.call("svdq_rms_norm_mx", x.data_ptr(), h, wide.data_ptr(), h + 11, None, 0, 1e-6, 5, h, codes.data_ptr(),
+                  scales.data_ptr(), wide.data_ptr(), h + 11, ops._raw_stream(x.device))
+        assert torch.equal(wide[:, :h], total) and (wide[:, h:] == 3).all()
+        assert torch.equal(codes.view(torch.uint8), q.codes.view(torch.uint8)) and torch.equal(scales, q.scales)
+
+
 def test_empty_batches():
     M = ms()
     w = M.quantize(data(64, 128), "nvfp4")
