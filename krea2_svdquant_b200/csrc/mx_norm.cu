@@ -2,8 +2,10 @@
 // scale per 32 columns):
 //   h = x + residual, rounded to its type and stored;   y = h * rsqrt(mean(h^2) + eps) * weight
 //   scale = 2^(floor(log2 max|y|) - 8) per 32 columns,  code = e4m3(y / scale)
-// The mean and y stay in fp32: y is rounded once, to its code.  The norm reads h as it is stored, so
-// a residual stream read back later gives the same norm.
+// The norm reads h as it is stored, so a residual stream read back later gives the same norm.  Squares
+// are summed in fp32 within a thread and in 64 bits over the row, the root is held as the sum of two
+// fp32 values, and h * weight is exact in fp32 for 16-bit types: y is rounded to fp32 once before it
+// is rounded to its code, so that hardly a code or a scale falls on the other side of a border.
 #include "mx_common.cuh"
 
 namespace svdq {
@@ -16,6 +18,7 @@ struct NormArgs {
   int64_t ldr;
   const void* weight;
   float eps;
+  double per_column;  // 1 / H
   int M, H, h_pad;
   uint8_t* codes;
   uint8_t* scales;
@@ -32,7 +35,7 @@ template <typename T, int THREADS, int PASSES, bool VEC>
 __global__ void __launch_bounds__(THREADS) rms_norm_mx_kernel(const NormArgs a) {
   constexpr int C = 32 / (int)sizeof(T);
   constexpr int kKeep = PASSES > 0 ? PASSES : 1;
-  __shared__ float part[THREADS / 32];
+  __shared__ double part[THREADS / 32];
   __shared__ __align__(16) T stage[VEC ? 1 : THREADS * C];
   pdl_wait();
   pdl_trigger();
@@ -91,26 +94,30 @@ __global__ void __launch_bounds__(THREADS) rms_norm_mx_kernel(const NormArgs a) 
       add(column(p), keep[0], res[0]);
     }
   }
-  float ss = f2_lo(ss2) + f2_hi(ss2);
+  double ss = (double)f2_lo(ss2) + (double)f2_hi(ss2);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
   if (lane == 0) part[tid >> 5] = ss;
   __syncthreads();
-  ss = 0.0f;
+  ss = 0.0;
 #pragma unroll
   for (int w = 0; w < THREADS / 32; ++w) ss += part[w];
-  const float inv = 1.0f / sqrtf(ss / (float)a.H + a.eps);
-  const uint64_t inv2 = f2_pack(inv, inv);
+  // 1 / sqrt(v) as hi + lo: hi = fp32 of it to a few ulp, lo = hi (1 - v hi^2) / 2 (a Newton step)
+  const double v = fma(ss, a.per_column, (double)a.eps);
+  const float hi = 1.0f / sqrtf((float)v);
+  const float lo = 0.5f * hi * (float)fma(-v, (double)hi * (double)hi, 1.0);
+  const uint64_t hi2 = f2_pack(hi, hi), lo2 = isfinite(hi) && hi != 0.0f ? f2_pack(lo, lo) : 0;
   auto encode = [&](int c, const T (&h)[C]) {
     alignas(32) T w[C];
     if (weight) load(weight, c, w);
     float y[C];
 #pragma unroll
     for (int i = 0; i < C; i += 2) {
-      uint64_t v = f2_mul(f2_pack(to_float(h[i]), to_float(h[i + 1])), inv2);
-      if (weight) v = f2_mul(v, f2_pack(to_float(w[i]), to_float(w[i + 1])));
-      y[i] = f2_lo(v);
-      y[i + 1] = f2_hi(v);
+      uint64_t p = f2_pack(to_float(h[i]), to_float(h[i + 1]));
+      if (weight) p = f2_mul(p, f2_pack(to_float(w[i]), to_float(w[i + 1])));
+      p = f2_fma(p, hi2, f2_mul(p, lo2));
+      y[i] = f2_lo(p);
+      y[i + 1] = f2_hi(p);
     }
     uint32_t amax = amax_bits_of(y);
     amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
@@ -187,6 +194,7 @@ extern "C" int svdq_rms_norm_mx(const void* x, int64_t ldx, const void* residual
   a.ldr = ldr;
   a.weight = weight;
   a.eps = eps;
+  a.per_column = 1.0 / H;
   a.M = M;
   a.H = H;
   a.h_pad = mx_k_pad(H);
