@@ -507,8 +507,10 @@ int svdq_mx_gemm(const void* a_codes, const void* a_scales, int a_format, const 
 
 /*
  * svdq_mx_quantize of x [M, K] (dtype, row stride ldx) to a_format, then svdq_mx_gemm with the weight,
- * in one call.  The activations' codes and scales are written to the workspace (256-byte aligned, at
- * least svdq_mx_linear_workspace_bytes(); needs no clearing; one call at a time per workspace).
+ * in one call.  Up to 4 tokens are quantised by the product itself, one launch without a workspace.
+ * Beyond that the activations' codes and scales are written to the workspace (256-byte aligned, at
+ * least svdq_mx_linear_workspace_bytes(), which is 0 up to 4 tokens; needs no clearing; one call at a
+ * time per workspace).  The same bits as the two calls.
  */
 size_t svdq_mx_linear_workspace_bytes(int M, int K, int a_format);
 int svdq_mx_linear(const void* x, int64_t ldx, int dtype, int a_format, const float* a_tensor_scale,

@@ -359,6 +359,61 @@ __device__ __forceinline__ void store_warp(T* row, int c, int K, T* stage, const
   __syncwarp();
 }
 
+// 16 codes: 8 bytes of 4-bit ones or 16 of 8-bit ones.
+template <int FMT>
+struct CodeWord {
+  using type = uint2;
+};
+template <>
+struct CodeWord<kMxfp8> {
+  using type = uint4;
+};
+
+// The codes of 16 columns (x is overwritten) and their block's scale byte.  An mx block is shared with
+// the neighbouring lane (lane ^ 1), so every lane of the warp takes part.
+template <typename T, int FMT>
+__device__ __forceinline__ typename CodeWord<FMT>::type encode_chunk(T (&x)[16], float g, const Nvfp4Unit* units,
+                                                                     uint32_t& byte) {
+  uint32_t amax = amax_bits_of(x);
+  if constexpr (FMT == kNvfp4) {  // nvfp4_codes takes -x
+    constexpr uint32_t kSigns = sizeof(T) == 2 ? 0x80008000u : 0x80000000u;
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) * 4; ++i) reinterpret_cast<uint32_t*>(x)[i] ^= kSigns;
+  } else {
+    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+  }
+  float v[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = to_float(x[i]);
+  if constexpr (FMT == kNvfp4) {
+    byte = nvfp4_scale_byte(amax, g);
+    return nvfp4_codes(v, amax, byte, units[byte], g);
+  } else {
+    byte = mx_scale_byte<FMT>(amax);
+    if (byte == 255u) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] = 0.0f;
+    }
+    scale_all(v, mx_inverse_scale(byte));
+    if constexpr (FMT == kMxfp4) {
+      return make_uint2(e2m1x8_satfinite(v), e2m1x8_satfinite(v + 8));
+    } else {
+      uint32_t w[4];
+      e4m3_words(v, w);
+      return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+}
+// The four scale bytes of a word, from the 4 (nvfp4) or 8 (mx) neighbouring lanes that have them.
+template <int FMT>
+__device__ __forceinline__ uint32_t scale_word(uint32_t byte) {
+  constexpr int kStep = FMT == kNvfp4 ? 1 : 2;  // lanes per block
+  uint32_t word = byte << (8 * (((threadIdx.x & 31) / kStep) & 3));
+  word |= __shfl_xor_sync(0xffffffffu, word, kStep);
+  word |= __shfl_xor_sync(0xffffffffu, word, 2 * kStep);
+  return word;
+}
+
 // Rows of a matrix start on boundaries of `align` bytes.
 inline bool rows_aligned(const void* p, int64_t ld, int elem_bytes, int align) {
   return reinterpret_cast<uintptr_t>(p) % align == 0 && (ld * elem_bytes) % align == 0;

@@ -7,8 +7,14 @@
 // where the tiles leave SMs idle, the CTAs of a cluster take a share of K each and add their fp32
 // partial tiles through distributed shared memory in rank order (the same result every time).
 // 6 warps: 0-3 epilogue, 4 TMA producer, 5 MMA and scale copies.
+//
+// For a few tokens the kernel can take the activations as they are: the epilogue warps, idle until
+// the end, quantise each stage's columns of the tokens into shared memory, in the layout that TMA would
+// have written.  Every CTA does so for its share of K; the work is small next to 128 weight rows, and
+// a launch and the wait for it are saved.
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "mx_gemm.cuh"
 
@@ -51,6 +57,8 @@ constexpr int kExtra = sizeof(SplitBars) + 1024;
 
 struct SplitArgs {
   MxOutput o;
+  MxInput in;
+  int k;
   int steps;    // stages of K in all
   int split;    // CTAs of the cluster, a share of K each
   int stages;   // ring depth
@@ -58,7 +66,16 @@ struct SplitArgs {
   int* err;
 };
 
-enum : int { kWaitSplitEmpty = 0x501, kWaitSplitFull = 0x511, kWaitSplitDone = 0x512, kWaitSplitEpi = 0x521 };
+enum : int { kWaitSplitEmpty = 0x501, kWaitSplitFull = 0x511, kWaitSplitDone = 0x512, kWaitSplitEpi = 0x521,
+             kWaitSplitQuant = 0x531 };
+
+__device__ __forceinline__ void mbar_arrive_cta(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+// Warps' worth of 16-column pieces in a stage of M tokens.
+template <int MODE>
+__host__ __device__ constexpr int fused_groups(int M) { return (M * (MxMode<MODE>::kStageCols / 16) + 31) / 32; }
 
 template <int MODE, int TN>
 struct SplitShape {
@@ -72,16 +89,79 @@ struct SplitShape {
   static constexpr int kStage = (kBytes + 1023) / 1024 * 1024;
   static constexpr int kSfw = TN < 32 ? 32 : TN;       // columns of tensor memory
   static constexpr int kSft = kSfw + 4 * MxMode<MODE>::kScaleTiles;
+  // bytes that TMA brings where the activations are quantised here
+  static constexpr int kTxFused = kTx - TN * 128 - kScale;
   static constexpr int kCols = kSft + 4 * MxMode<MODE>::kScaleTiles <= 64 ? 64 : kSft + 16 <= 128 ? 128 : 256;
 };
 
-template <int MODE, int TN>
+// The activations of stages s0 .. s1 - 1, quantised by warps 0-3.  A lane takes 16 columns of a token;
+// `groups` warps' worth of them make a stage, and the warps take the groups of all stages in turn, each
+// with its next group's columns on the way while it works on one.
+template <int MODE, typename T>
+__device__ __forceinline__ void quantize_stages(const SplitArgs& a, SplitBars* bars, uint8_t* ring, int stage_bytes,
+                                                int tok, int scale, Nvfp4Unit* units, int s0, int s1,
+                                                volatile int* abort_flag) {
+  constexpr int kFmt = MODE == kModeNvfp4 ? kNvfp4 : MODE == kModeMxfp4 ? kMxfp4 : kMxfp8;
+  constexpr int kChunks = MxMode<MODE>::kStageCols / 16;  // per token and stage
+  constexpr int kLanes = kFmt == kNvfp4 ? 4 : 8;          // per word of scales
+  using Codes = typename CodeWord<kFmt>::type;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int groups = fused_groups<MODE>(a.o.M);
+  const float g = kFmt == kNvfp4 && a.o.a_scale ? *a.o.a_scale : 1.0f;
+  auto load = [&](int s, int group, T (&x)[16]) {
+    const int item = group * 32 + lane, m = item / kChunks;
+    const int c = m < a.o.M && s < s1 ? s * MxMode<MODE>::kStageCols + item % kChunks * 16 : a.k;
+    const T* row = static_cast<const T*>(a.in.x) + (m < a.o.M ? (size_t)m * a.in.ldx : 0);
+    if (!a.in.vec) {
+      load_shifted(row, c, a.k, x);
+    } else if (c < a.k) {
+      load_vec(row + c, x);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) x[j] = from_float<T>(0.0f);
+    }
+  };
+  alignas(32) T x[16];
+  load(s0 + warp / groups, warp % groups, x);
+  if constexpr (kFmt == kNvfp4) {
+    units[threadIdx.x] = nvfp4_unit<significant_bits<T>()>(threadIdx.x, g);
+    asm volatile("bar.sync 1, 128;" ::: "memory");  // warps 0-3
+  }
+  for (int q = warp; q < (s1 - s0) * groups; q += 4) {
+    alignas(32) T next[16];
+    load(s0 + (q + 4) / groups, (q + 4) % groups, next);
+    uint32_t byte;
+    const Codes codes = encode_chunk<T, kFmt>(x, g, units, byte);
+    const uint32_t word = scale_word<kFmt>(byte);
+    const int turn = q / groups, stage = turn % a.stages;
+    const uint32_t phase = (uint32_t)(turn / a.stages) & 1u;
+    if (!warp_spin_wait(smem_u32(&bars->empty[stage]), phase ^ 1u, abort_flag, a.err, kWaitSplitQuant)) break;
+    uint8_t* at = ring + (size_t)stage * stage_bytes;
+    const int item = q % groups * 32 + lane, m = item / kChunks, c = item % kChunks;
+    if (m < a.o.M) {
+      // 128-byte rows in 16-byte pieces, piece p of row m at p ^ (m % 8) (the 128-byte swizzle)
+      const int off = c * (int)sizeof(Codes);
+      *reinterpret_cast<Codes*>(at + tok + m * 128 + ((((off >> 4) ^ (m & 7)) << 4) | (off & 15))) = codes;
+      if (c % kLanes == 0) *reinterpret_cast<uint32_t*>(at + scale + (c / kLanes) * 512 + m * 16) = word;
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive_cta(smem_u32(&bars->full[stage]));
+#pragma unroll
+    for (int j = 0; j < 16; ++j) x[j] = next[j];
+  }
+}
+
+// X: the activations' type where they are quantised here, void where they come as codes and scales.
+template <int MODE, int TN, typename X>
 __global__ void __launch_bounds__(kSplitThreads)
     mx_gemm_split_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap t_map,
                          const __grid_constant__ CUtensorMap sw_map, const __grid_constant__ CUtensorMap st_map,
                          const __grid_constant__ SplitArgs a) {
   using S = SplitShape<MODE, TN>;
   using Mode = MxMode<MODE>;
+  constexpr bool kFused = !std::is_void<X>::value;
+  __shared__ __align__(16) Nvfp4Unit units[kFused && MODE == kModeNvfp4 ? 128 : 1];
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t pad = (1024u - (raw & 1023u)) & 1023u;
@@ -96,7 +176,8 @@ __global__ void __launch_bounds__(kSplitThreads)
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < a.stages; ++s) {
-      mbar_init(smem_u32(&bars->full[s]), 1);
+      // the producer, and the groups of activations that are quantised here
+      mbar_init(smem_u32(&bars->full[s]), 1 + (kFused ? fused_groups<MODE>(a.o.M) : 0));
       mbar_init(smem_u32(&bars->empty[s]), 1);
     }
     mbar_init(smem_u32(&bars->done), 1);
@@ -105,9 +186,11 @@ __global__ void __launch_bounds__(kSplitThreads)
   }
   if (warp == 4 && lane == 0) {
     prefetch_tma_desc(&w_map);
-    prefetch_tma_desc(&t_map);
     prefetch_tma_desc(&sw_map);
-    prefetch_tma_desc(&st_map);
+    if (!kFused) {
+      prefetch_tma_desc(&t_map);
+      prefetch_tma_desc(&st_map);
+    }
   }
   if (warp == 5) {
     tmem_alloc_1(smem_u32(&bars->tmem_base), S::kCols);
@@ -129,11 +212,13 @@ __global__ void __launch_bounds__(kSplitThreads)
       if (!(ok = warp_spin_wait(smem_u32(&bars->empty[stage]), phase ^ 1u, abort_flag, a.err, kWaitSplitEmpty))) break;
       const uint32_t bar = smem_u32(&bars->full[stage]), at = base + (uint32_t)(stage * S::kStage);
       if (elect_one()) {
-        mbar_arrive_expect_tx(bar, S::kTx);
+        mbar_arrive_expect_tx(bar, kFused ? S::kTxFused : S::kTx);
         tma_load_2d(at, &w_map, bar, s * 128, n0);
         tma_load_3d(at + S::kScaleW, &sw_map, bar, 0, s * Mode::kScaleTiles, n0 / 128);
-        tma_load_2d(at + S::kTok, &t_map, bar, s * 128, m0);
-        tma_load_3d(at + S::kScaleT, &st_map, bar, 0, s * Mode::kScaleTiles, m0 / 128);
+        if (!kFused) {
+          tma_load_2d(at + S::kTok, &t_map, bar, s * 128, m0);
+          tma_load_3d(at + S::kScaleT, &st_map, bar, 0, s * Mode::kScaleTiles, m0 / 128);
+        }
       }
       __syncwarp();
       filled |= 1u << stage;
@@ -180,6 +265,11 @@ __global__ void __launch_bounds__(kSplitThreads)
         atomicCAS(a.err, 0, kWaitSplitDone);
       }
     }
+    __syncwarp();
+  }
+  if constexpr (kFused) {
+    if (warp < 4)
+      quantize_stages<MODE, X>(a, bars, smem_raw + pad, S::kStage, S::kTok, S::kScaleT, units, s0, s1, abort_flag);
     __syncwarp();
   }
   // epilogue: warp w holds weight rows 32 w .. 32 w + 31, one per lane, and every token's column
@@ -292,10 +382,10 @@ struct SplitPlan {
 // nvfp4 at 128 tokens is bound by its scale copies.  Measured at N 6144, K 6144 with one CTA a tile.
 constexpr float kStageUs[3][4] = {{.30f, .33f, .44f, .64f}, {.26f, .28f, .38f, .50f}, {.24f, .26f, .36f, .43f}};
 
-template <int MODE, int TN>
+template <int MODE, int TN, typename X>
 int plan_split(const MxGemm& g, SplitPlan* p) {
   using S = SplitShape<MODE, TN>;
-  auto kern = mx_gemm_split_kernel<MODE, TN>;
+  auto kern = mx_gemm_split_kernel<MODE, TN, X>;
   cudaError_t ce = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kRoomOne + kExtra);
   if (ce == cudaSuccess)
     ce = cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
@@ -321,24 +411,31 @@ int plan_split(const MxGemm& g, SplitPlan* p) {
   return SVDQ_OK;
 }
 
-template <int MODE, int TN>
+template <int MODE, int TN, typename X>
 int launch_split(const MxGemm& g, const SplitPlan& p) {
   using S = SplitShape<MODE, TN>;
   CUtensorMap w, t, sw, st;
   int e;
   const bool spread = MODE == kModeW4A8;
   if ((e = make_code_map(&w, g.w_codes, g.w_fmt, spread, g.o.N, g.k_pad, kRows))) return e;
-  if ((e = make_code_map(&t, g.a_codes, g.a_fmt, false, g.o.M, g.k_pad, TN))) return e;
   if ((e = make_scale_map(&sw, g.w_scales, g.w_fmt, g.o.N, g.k_pad, MxMode<MODE>::kScaleTiles, 1))) return e;
-  if ((e = make_scale_map(&st, g.a_scales, g.a_fmt, g.o.M, g.k_pad, MxMode<MODE>::kScaleTiles, 1))) return e;
+  if (std::is_void<X>::value) {
+    if ((e = make_code_map(&t, g.a_codes, g.a_fmt, false, g.o.M, g.k_pad, TN))) return e;
+    if ((e = make_scale_map(&st, g.a_scales, g.a_fmt, g.o.M, g.k_pad, MxMode<MODE>::kScaleTiles, 1))) return e;
+  } else {  // not read
+    t = w;
+    st = sw;
+  }
   SplitArgs a{};
   a.o = g.o;
+  a.in = g.in;
+  a.k = g.k;
   a.err = g.err;
   a.steps = p.steps;
   a.n_tiles = p.n_tiles;
   a.split = p.split;
   a.stages = p.stages;
-  return launch_pdl("svdq_mx_gemm launch", mx_gemm_split_kernel<MODE, TN>, dim3((unsigned)(p.tiles * p.split)),
+  return launch_pdl("svdq_mx_gemm launch", mx_gemm_split_kernel<MODE, TN, X>, dim3((unsigned)(p.tiles * p.split)),
                     dim3(kSplitThreads), (size_t)a.stages * S::kStage + kExtra, g.stream, a.split, w, t, sw, st, a);
 }
 
@@ -349,14 +446,24 @@ template <int MODE, int TN>
 int choose(const MxGemm& g) {
   constexpr float kPairUs[3] = {.42f, .40f, .36f};
   SplitPlan p;
-  const int e = plan_split<MODE, TN>(g, &p);
+  const int e = plan_split<MODE, TN, void>(g, &p);
   if (e) return e;
   const int pairs = num_sms() / 2, tiles = ((g.o.M + 255) / 256) * ((g.o.N + 255) / 256);
   const float us = (float)((tiles + pairs - 1) / pairs) * p.steps * kPairUs[MODE];
-  return us < p.us ? launch_mx_gemm_pair(g) : launch_split<MODE, TN>(g, p);
+  return us < p.us ? launch_mx_gemm_pair(g) : launch_split<MODE, TN, void>(g, p);
+}
+template <int MODE, typename X>
+int launch_fused(const MxGemm& g) {
+  SplitPlan p;
+  const int e = plan_split<MODE, 16, X>(g, &p);
+  return e ? e : launch_split<MODE, 16, X>(g, p);
 }
 template <int MODE>
 int choose_tokens(const MxGemm& g) {
+  if (g.in.x)
+    return g.in.dtype == SVDQ_BF16   ? launch_fused<MODE, __nv_bfloat16>(g)
+           : g.in.dtype == SVDQ_FP16 ? launch_fused<MODE, __half>(g)
+                                     : launch_fused<MODE, float>(g);
   if (g.o.M <= 16) return choose<MODE, 16>(g);
   if (g.o.M <= 32) return choose<MODE, 32>(g);
   if (g.o.M <= 64) return choose<MODE, 64>(g);
@@ -366,39 +473,31 @@ int choose_tokens(const MxGemm& g) {
 }  // namespace
 }  // namespace svdq
 
-extern "C" int svdq_mx_gemm(const void* a_codes, const void* a_scales, int a_format, const float* a_tensor_scale,
-                            const void* w_codes, const void* w_scales, int w_format, const float* w_tensor_scale,
-                            const void* bias, void* out, int out_dtype, int64_t ldo, int M, int N, int K,
-                            cudaStream_t stream) {
-  using namespace svdq;
-  SVDQ_REQUIRE((a_format == w_format && (a_format == kNvfp4 || a_format == kMxfp4)) ||
-                   (a_format == kMxfp8 && w_format == kMxfp4),
+namespace svdq {
+namespace {
+
+// Checks a product's arguments (the activations as codes and scales, or g.in) and runs it.
+int mx_product(MxGemm& g, int K) {
+  const int M = g.o.M, N = g.o.N;
+  SVDQ_REQUIRE((g.a_fmt == g.w_fmt && (g.a_fmt == kNvfp4 || g.a_fmt == kMxfp4)) ||
+                   (g.a_fmt == kMxfp8 && g.w_fmt == kMxfp4),
                "svdq_mx_gemm: operands are nvfp4 x nvfp4, mxfp4 x mxfp4 or mxfp8 x mxfp4 (activations x weight)");
-  SVDQ_REQUIRE(dtype_ok(out_dtype), "svdq_mx_gemm: out must be bf16, fp16 or fp32");
-  SVDQ_REQUIRE(M >= 0 && N > 0 && K > 0 && ldo >= N, "svdq_mx_gemm: bad M/N/K/ldo");
-  SVDQ_REQUIRE((!a_tensor_scale && !w_tensor_scale) || a_format == kNvfp4,
-               "svdq_mx_gemm: only nvfp4 operands have tensor scales");
+  SVDQ_REQUIRE(dtype_ok(g.o.out_dtype), "svdq_mx_gemm: out must be bf16, fp16 or fp32");
+  SVDQ_REQUIRE(M >= 0 && N > 0 && K > 0 && g.o.ldo >= N, "svdq_mx_gemm: bad M/N/K/ldo");
+  SVDQ_REQUIRE((!g.o.a_scale && !g.o.w_scale) || g.a_fmt == kNvfp4, "svdq_mx_gemm: only nvfp4 operands have tensor scales");
   if (M == 0) return SVDQ_OK;
-  SVDQ_REQUIRE(a_codes && a_scales && w_codes && w_scales && out, "svdq_mx_gemm: null pointer");
-  SVDQ_REQUIRE(((reinterpret_cast<uintptr_t>(a_codes) | reinterpret_cast<uintptr_t>(a_scales) |
-                 reinterpret_cast<uintptr_t>(w_codes) | reinterpret_cast<uintptr_t>(w_scales)) & 31u) == 0,
+  SVDQ_REQUIRE((g.in.x || (g.a_codes && g.a_scales)) && g.w_codes && g.w_scales && g.o.out, "svdq_mx_gemm: null pointer");
+  SVDQ_REQUIRE(((reinterpret_cast<uintptr_t>(g.a_codes) | reinterpret_cast<uintptr_t>(g.a_scales) |
+                 reinterpret_cast<uintptr_t>(g.w_codes) | reinterpret_cast<uintptr_t>(g.w_scales)) & 31u) == 0,
                "svdq_mx_gemm: codes and scales must be 32-byte aligned");
-  SVDQ_REQUIRE((reinterpret_cast<uintptr_t>(out) % dtype_bytes(out_dtype)) == 0 &&
-                   (reinterpret_cast<uintptr_t>(bias) & 1u) == 0,
+  SVDQ_REQUIRE((reinterpret_cast<uintptr_t>(g.o.out) % dtype_bytes(g.o.out_dtype)) == 0 &&
+                   (reinterpret_cast<uintptr_t>(g.o.bias) & 1u) == 0,
                "svdq_mx_gemm: out and bias must be aligned to their elements");
   if (M > (1 << 24) || N > (1 << 24) || K > (1 << 28))
     return set_error(SVDQ_ERR_UNSUPPORTED, "svdq_mx_gemm: M and N up to 2^24, K up to 2^28");
-  MxGemm g{};
-  g.mode = a_format == kNvfp4 ? kModeNvfp4 : a_format == kMxfp4 ? kModeMxfp4 : kModeW4A8;
-  g.a_codes = a_codes;
-  g.a_scales = a_scales;
-  g.w_codes = w_codes;
-  g.w_scales = w_scales;
-  g.a_fmt = a_format;
-  g.w_fmt = w_format;
+  g.mode = g.a_fmt == kNvfp4 ? kModeNvfp4 : g.a_fmt == kMxfp4 ? kModeMxfp4 : kModeW4A8;
+  g.k = K;
   g.k_pad = mx_k_pad(K);
-  g.o = MxOutput{a_tensor_scale, w_tensor_scale, static_cast<const __nv_bfloat16*>(bias), out, ldo, out_dtype, M, N};
-  g.stream = stream;
   g.err = device_error_word();
   if (!g.err) return set_error(SVDQ_ERR_CUDA, "svdq_mx_gemm: device error word unavailable");
   if (g.mode == kModeNvfp4) return choose_tokens<kModeNvfp4>(g);
@@ -406,12 +505,31 @@ extern "C" int svdq_mx_gemm(const void* a_codes, const void* a_scales, int a_for
 }
 
 // Workspace of svdq_mx_linear: the codes, then the scales from the next 256-byte boundary.
-static size_t mx_code_bytes(int M, int K, int fmt) {
-  return ((size_t)M * svdq::mx_row_bytes(fmt, svdq::mx_k_pad(K)) + 255) / 256 * 256;
+size_t mx_code_bytes(int M, int K, int fmt) { return ((size_t)M * mx_row_bytes(fmt, mx_k_pad(K)) + 255) / 256 * 256; }
+
+}  // namespace
+}  // namespace svdq
+
+extern "C" int svdq_mx_gemm(const void* a_codes, const void* a_scales, int a_format, const float* a_tensor_scale,
+                            const void* w_codes, const void* w_scales, int w_format, const float* w_tensor_scale,
+                            const void* bias, void* out, int out_dtype, int64_t ldo, int M, int N, int K,
+                            cudaStream_t stream) {
+  using namespace svdq;
+  MxGemm g{};
+  g.a_codes = a_codes;
+  g.a_scales = a_scales;
+  g.a_fmt = a_format;
+  g.w_codes = w_codes;
+  g.w_scales = w_scales;
+  g.w_fmt = w_format;
+  g.o = MxOutput{a_tensor_scale, w_tensor_scale, static_cast<const __nv_bfloat16*>(bias), out, ldo, out_dtype, M, N};
+  g.stream = stream;
+  return mx_product(g, K);
 }
 
 extern "C" size_t svdq_mx_linear_workspace_bytes(int M, int K, int a_format) {
-  if (M <= 0 || K <= 0 || !svdq::mx_format_ok(a_format) || M > (1 << 30) || K > (1 << 30)) return 0;
+  using namespace svdq;
+  if (M <= kMaxFusedTokens || K <= 0 || !mx_format_ok(a_format) || M > (1 << 30) || K > (1 << 30)) return 0;
   return mx_code_bytes(M, K, a_format) + svdq_mx_scale_bytes(M, K, a_format);
 }
 
@@ -421,18 +539,28 @@ extern "C" int svdq_mx_linear(const void* x, int64_t ldx, int dtype, int a_forma
                               void* workspace, size_t workspace_bytes, cudaStream_t stream) {
   using namespace svdq;
   SVDQ_REQUIRE(mx_format_ok(a_format), "svdq_mx_linear: unknown activation format");
-  SVDQ_REQUIRE(M >= 0 && K > 0, "svdq_mx_linear: bad M/K");
-  SVDQ_REQUIRE(M == 0 || (workspace && (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0 &&
-                          workspace_bytes >= svdq_mx_linear_workspace_bytes(M, K, a_format)),
+  SVDQ_REQUIRE(dtype_ok(dtype), "svdq_mx_linear: x must be bf16, fp16 or fp32");
+  SVDQ_REQUIRE(M >= 0 && K > 0 && ldx >= K, "svdq_mx_linear: bad M/K/ldx");
+  SVDQ_REQUIRE(x || M == 0, "svdq_mx_linear: null pointer");
+  SVDQ_REQUIRE((reinterpret_cast<uintptr_t>(x) % dtype_bytes(dtype)) == 0, "svdq_mx_linear: x must be aligned to its elements");
+  MxGemm g{};
+  g.a_fmt = a_format;
+  g.w_codes = w_codes;
+  g.w_scales = w_scales;
+  g.w_fmt = w_format;
+  g.o = MxOutput{a_tensor_scale, w_tensor_scale, static_cast<const __nv_bfloat16*>(bias), out, ldo, out_dtype, M, N};
+  g.stream = stream;
+  if (M <= kMaxFusedTokens) {  // one launch
+    g.in = MxInput{x, ldx, dtype, K % 16 == 0 && rows_aligned(x, ldx, dtype_bytes(dtype), 32)};
+    return mx_product(g, K);
+  }
+  SVDQ_REQUIRE(workspace && (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0 &&
+                   workspace_bytes >= svdq_mx_linear_workspace_bytes(M, K, a_format),
                "svdq_mx_linear: workspace must be 256-byte aligned and hold svdq_mx_linear_workspace_bytes()");
   uint8_t* codes = static_cast<uint8_t*>(workspace);
-  uint8_t* scales = M > 0 ? codes + mx_code_bytes(M, K, a_format) : nullptr;
-  // the product's arguments are checked before anything is launched
-  int st = svdq_mx_gemm(codes, scales, a_format, a_tensor_scale, w_codes, w_scales, w_format, w_tensor_scale, bias, out,
-                        out_dtype, ldo, 0, N, K, stream);
-  if (!st) st = svdq_mx_quantize(x, ldx, dtype, M, K, a_format, a_tensor_scale, codes, scales, stream);
-  if (!st)
-    st = svdq_mx_gemm(codes, scales, a_format, a_tensor_scale, w_codes, w_scales, w_format, w_tensor_scale, bias, out,
-                      out_dtype, ldo, M, N, K, stream);
-  return st;
+  uint8_t* scales = codes + mx_code_bytes(M, K, a_format);
+  g.a_codes = codes;
+  g.a_scales = scales;
+  const int st = svdq_mx_quantize(x, ldx, dtype, M, K, a_format, a_tensor_scale, codes, scales, stream);
+  return st ? st : mx_product(g, K);
 }

@@ -26,15 +26,6 @@ __device__ __forceinline__ uint32_t div_by(const FastDiv& f, uint32_t n) {
 // Chunks of 16 elements per thread: 64 bytes in flight.
 template <typename T>
 __host__ __device__ constexpr int unroll_of() { return sizeof(T) == 2 ? 2 : 1; }
-template <int FMT>
-struct CodeWord {
-  using type = uint2;  // 16 codes
-};
-template <>
-struct CodeWord<kMxfp8> {
-  using type = uint4;
-};
-
 struct QuantArgs {
   const void* x;
   int64_t ldx;
@@ -55,47 +46,15 @@ struct QuantArgs {
 template <typename T, int FMT>
 __device__ __forceinline__ void quantize_chunk(const QuantArgs& a, T (&x)[16], uint32_t id, int row, int chunk,
                                                bool live, float g, const Nvfp4Unit* units) {
-  const int lane = threadIdx.x & 31;
-  uint32_t amax = amax_bits_of(x);
-  if constexpr (FMT == kNvfp4) {  // nvfp4_codes takes -x
-    constexpr uint32_t kSigns = sizeof(T) == 2 ? 0x80008000u : 0x80000000u;
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(T) * 4; ++i) reinterpret_cast<uint32_t*>(x)[i] ^= kSigns;
-  } else {
-    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-  }
-  float v[16];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) v[i] = to_float(x[i]);
-  uint32_t byte = 0;
-  if (live) {
-    uint8_t* codes = a.codes + (size_t)row * mx_row_bytes(FMT, (int)a.per_row.d * 16) + chunk * (FMT == kMxfp8 ? 16 : 8);
-    if constexpr (FMT == kNvfp4) {
-      byte = nvfp4_scale_byte(amax, g);
-      *reinterpret_cast<uint2*>(codes) = nvfp4_codes(v, amax, byte, units[byte], g);
-    } else {
-      byte = mx_scale_byte<FMT>(amax);
-      if (byte == 255u) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = 0.0f;
-      }
-      scale_all(v, mx_inverse_scale(byte));
-      if constexpr (FMT == kMxfp4) {
-        *reinterpret_cast<uint2*>(codes) = make_uint2(e2m1x8_satfinite(v), e2m1x8_satfinite(v + 8));
-      } else {
-        uint32_t w[4];
-        e4m3_words(v, w);
-        *reinterpret_cast<uint4*>(codes) = make_uint4(w[0], w[1], w[2], w[3]);
-      }
-    }
-  }
-  constexpr int kStep = FMT == kNvfp4 ? 1 : 2;  // lanes per block
-  uint32_t word = byte << (8 * ((lane / kStep) & 3));
-  word |= __shfl_xor_sync(0xffffffffu, word, kStep);
-  word |= __shfl_xor_sync(0xffffffffu, word, 2 * kStep);
-  if (id < a.chunks && lane % (4 * kStep) == 0)
-    *reinterpret_cast<uint32_t*>(a.scales + mx_scale_word(row, chunk / (4 * kStep), (int)a.per_row.d / (4 * kStep))) =
-        word;
+  using Codes = typename CodeWord<FMT>::type;
+  uint32_t byte;
+  const Codes codes = encode_chunk<T, FMT>(x, g, units, byte);
+  if (live)
+    reinterpret_cast<Codes*>(a.codes + (size_t)row * mx_row_bytes(FMT, (int)a.per_row.d * 16))[chunk] = codes;
+  constexpr int kLanes = FMT == kNvfp4 ? 4 : 8;  // per word of scales
+  const uint32_t word = scale_word<FMT>(live ? byte : 0u);
+  if (id < a.chunks && (threadIdx.x & 31) % kLanes == 0)
+    *reinterpret_cast<uint32_t*>(a.scales + mx_scale_word(row, chunk / kLanes, (int)a.per_row.d / kLanes)) = word;
 }
 
 // A CTA takes kThreads * kUnroll neighbouring chunks at a time.  For nvfp4 it stays for a share of

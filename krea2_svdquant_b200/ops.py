@@ -788,11 +788,14 @@ def _(a_codes, a_scales, a_fmt, a_tensor_scale, w_codes, w_scales, w_fmt, w_tens
     return a_codes.new_empty((a_codes.shape[0], w_codes.shape[0]), dtype=out_dtype)
 
 
+MX_FUSED_TOKENS = 4  # svdq_mx_linear quantises up to this many tokens inside the product
+
+
 @_op("mx_linear")
 def mx_linear(x: Tensor, a_fmt: str, a_tensor_scale: Optional[Tensor], w_codes: Tensor, w_scales: Tensor, w_fmt: str,
               w_tensor_scale: Optional[Tensor], bias: Optional[Tensor], out_dtype: torch.dtype) -> Tensor:
-    """``mx_gemm(*mx_quantize(x, a_fmt, a_tensor_scale), ...)`` in one call (``svdq_mx_linear``): the
-    activations' codes and scales live in a workspace."""
+    """``mx_gemm(*mx_quantize(x, a_fmt, a_tensor_scale), ...)`` in one call (``svdq_mx_linear``): up to
+    ``MX_FUSED_TOKENS`` tokens are quantised by the product itself, beyond that into a workspace."""
     dev = _mx_device("mx_linear", x, a_tensor_scale, w_codes, w_scales, w_tensor_scale, bias)
     a_code = _mx_format("mx_linear", a_fmt)
     m, k, ld = _mx_rows("mx_linear", x)
@@ -803,12 +806,15 @@ def mx_linear(x: Tensor, a_fmt: str, a_tensor_scale: Optional[Tensor], w_codes: 
     _mx_gemm_check("mx_linear", a_fmt, w_fmt, n, bias, out_dtype)
     out = x.new_empty((m, n), dtype=out_dtype)
     if m and n:
-        codes = m * mx_k_pad(k) // (1 if a_fmt == "mxfp8" else 2)
-        ws = x.new_empty((codes + 1024 + mx_scales_numel(m, k, a_fmt),), dtype=torch.uint8)
+        ws, n_ws = None, 0
+        if m > MX_FUSED_TOKENS:
+            codes = m * mx_k_pad(k) // (1 if a_fmt == "mxfp8" else 2)
+            n_ws = (codes + 255) // 256 * 256 + mx_scales_numel(m, k, a_fmt)
+            ws = x.new_empty(n_ws, dtype=torch.uint8)
         with _on(dev):
             _lib.call("svdq_mx_linear", x.data_ptr(), ld, _DT[x.dtype], a_code, _ptr(a_tensor_scale),
                       w_codes.data_ptr(), w_scales.data_ptr(), w_code, _ptr(w_tensor_scale), _ptr(bias),
-                      out.data_ptr(), _DT[out_dtype], n, m, n, k, ws.data_ptr(), ws.shape[0], _raw_stream(dev))
+                      out.data_ptr(), _DT[out_dtype], n, m, n, k, _ptr(ws), n_ws, _raw_stream(dev))
     return out
 
 

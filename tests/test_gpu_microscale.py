@@ -408,6 +408,27 @@ def test_norm_in_place_through_the_c_abi():
         assert torch.equal(codes.view(torch.uint8), q.codes.view(torch.uint8)) and torch.equal(scales, q.scales)
 
 
+@pytest.mark.parametrize("act,w_fmt", PRODUCTS)
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+@pytest.mark.parametrize("m,n,k,cut", [(1, 128, 128, 0), (1, 300, 6144, 0), (3, 1537, 1030, 0), (2, 64, 77, 4), (4, 200, 640, 16),
+                                       (4, 520, 2048, 0), (4, 129, 1, 2), (3, 2000, 999, 1), (5, 300, 700, 0)])
+def test_few_tokens_quantised_by_the_product(act, w_fmt, dtype, m, n, k, cut):
+    """Up to 4 tokens: one launch, the same bits as the quantisation and the product one after the other."""
+    M = ms()
+    x, w = data(m, k, DTYPES[dtype], seed=m, cut=cut), data(n, k, seed=n, scale=0.1)
+    g = torch.tensor([0.0213], device="cuda") if act == "nvfp4" else None
+    wq = M.quantize(w, w_fmt, tensor_scale=M.tensor_scale(w) if act == "nvfp4" else None)
+    bias = data(1, n, torch.bfloat16, seed=3)[0].contiguous()
+    a = M.quantize(x, act, tensor_scale=g)
+    y = M.linear(x, wq, bias, act=act, act_scale=g)
+    assert y.dtype == x.dtype and torch.equal(y, M.matmul(a, wq, bias, out_dtype=x.dtype))
+    check_product(y, operand_values(a), operand_values(wq), bias, DTYPES[dtype])
+    x[0, k // 2] = float("inf")
+    y2 = M.linear(x, wq, bias, act=act, act_scale=g)
+    assert torch.isnan(y2[0]).all() and torch.equal(y2[1:], y[1:])
+    no_device_error()
+
+
 def test_empty_batches():
     M = ms()
     w = M.quantize(data(64, 128), "nvfp4")

@@ -146,14 +146,18 @@ def test_c_abi_refusals():
     assert gemm(m=1 << 25) == 2
     assert gemm(m=0) == 0
 
-    def lin(x=p, a_fmt=0, w_fmt=0, ws=p, nws=1 << 20, m=4, n=64, ldx=64, ldo=64, w=p):
-        return L.svdq_mx_linear(x, ldx, 0, a_fmt, None, w, p, w_fmt, None, None, p, 0, ldo, m, n, 64, ws, nws, None)
+    def lin(x=p, a_fmt=0, w_fmt=0, ws=p, nws=1 << 20, m=4, n=64, ldx=64, ldo=64, w=p, dt=0):
+        return L.svdq_mx_linear(x, ldx, dt, a_fmt, None, w, p, w_fmt, None, None, p, 0, ldo, m, n, 64, ws, nws, None)
 
-    assert lin(a_fmt=5) == 1 and lin(ws=None) == 1 and lin(ws=ctypes.c_void_p(4096 + 16)) == 1
-    assert lin(nws=L.svdq_mx_linear_workspace_bytes(4, 64, 0) - 1) == 1 and "workspace" in last()
+    need = L.svdq_mx_linear_workspace_bytes
+    assert lin(a_fmt=5) == 1 and lin(m=5, ws=None) == 1 and lin(m=5, ws=ctypes.c_void_p(4096 + 16)) == 1
+    assert lin(m=5, nws=need(5, 64, 0) - 1) == 1 and "workspace" in last()
     assert lin(w_fmt=1) == 1 and "operands" in last()
-    assert lin(ldo=60) == 1 and lin(n=0) == 1 and lin(ldx=60) == 1 and lin(x=None) == 1 and lin(m=0) == 0
-    assert L.svdq_mx_linear_workspace_bytes(0, 64, 0) == 0 and L.svdq_mx_linear_workspace_bytes(4, 64, 9) == 0
+    assert lin(x=ctypes.c_void_p(4097)) == 1 and lin(w=None) == 1 and lin(w=ctypes.c_void_p(4096 + 16)) == 1
+    assert lin(ldo=60) == 1 and lin(n=0) == 1 and lin(ldx=60) == 1 and lin(x=None) == 1 and lin(dt=7) == 1
+    assert lin(m=0) == 0 and lin(m=0, ws=None) == 0
+    assert need(0, 64, 0) == 0 and need(4, 64, 0) == 0 and need(5, 64, 9) == 0 and need(5, 64, 0) == 512 + 128 * 8
+    assert need(300, 1000, 2) == 300 * 1024 + 384 * 32
 
     def norm(x=p, r=None, s=None, dt=0, eps=1e-6, m=4, h=64, ldx=64, ldr=64, lds=64):
         return L.svdq_rms_norm_mx(x, ldx, r, ldr, None, dt, eps, m, h, p, p, s, lds, None)
