@@ -619,10 +619,10 @@ def mx_scales_numel(rows: int, k: int, fmt: str) -> int:
     return (rows + 127) // 128 * 128 * (mx_k_pad(k) // MX_BLOCK[fmt])
 
 
-def _mx_codes_like(x: Tensor, rows: int, k: int, fmt: str) -> Tensor:
+def _mx_codes(rows: int, k: int, fmt: str, dev: torch.device) -> Tensor:
     if fmt == "mxfp8":
-        return x.new_empty((rows, mx_k_pad(k)), dtype=torch.float8_e4m3fn)
-    return x.new_empty((rows, mx_k_pad(k) // 2), dtype=torch.uint8)
+        return _matrix(rows, mx_k_pad(k), torch.float8_e4m3fn, dev)
+    return _matrix(rows, mx_k_pad(k) // 2, torch.uint8, dev)
 
 
 # The checks below cost a small call a few us of host time, so they build their messages only to raise.
@@ -686,6 +686,11 @@ def _ptr(t: Optional[Tensor]):
     return None if t is None else t.data_ptr()
 
 
+def _matrix(rows: int, cols: int, dtype: torch.dtype, dev: torch.device) -> Tensor:
+    """An uninitialised contiguous matrix (``empty_strided`` takes 0.5-0.9 us less than ``empty``)."""
+    return torch.empty_strided((rows, cols), (cols, 1), dtype=dtype, device=dev)
+
+
 @_op("mx_quantize")
 def mx_quantize(x: Tensor, fmt: str, tensor_scale: Optional[Tensor]) -> tuple[Tensor, Tensor]:
     """``x [M, K]`` (bf16, fp16 or fp32, unit column stride) as block-scaled codes and scales
@@ -696,8 +701,8 @@ def mx_quantize(x: Tensor, fmt: str, tensor_scale: Optional[Tensor]) -> tuple[Te
     m, k, ld = _mx_rows("mx_quantize", x)
     if tensor_scale is not None:
         _mx_check_tensor_scale("mx_quantize", fmt, tensor_scale)
-    codes = _mx_codes_like(x, m, k, fmt)
-    scales = x.new_empty((mx_scales_numel(m, k, fmt),), dtype=torch.uint8)
+    codes = _mx_codes(m, k, fmt, dev)
+    scales = x.new_empty(mx_scales_numel(m, k, fmt), dtype=torch.uint8)
     if m:
         with _on(dev):
             _lib.call("svdq_mx_quantize", x.data_ptr(), ld, _DT[x.dtype], m, k, code, _ptr(tensor_scale),
@@ -708,7 +713,7 @@ def mx_quantize(x: Tensor, fmt: str, tensor_scale: Optional[Tensor]) -> tuple[Te
 @mx_quantize.register_fake
 def _(x, fmt, tensor_scale):
     m, k = x.shape
-    return _mx_codes_like(x, m, k, fmt), x.new_empty((mx_scales_numel(m, k, fmt),), dtype=torch.uint8)
+    return _mx_codes(m, k, fmt, x.device), x.new_empty((mx_scales_numel(m, k, fmt),), dtype=torch.uint8)
 
 
 @_op("mx_dequantize")
@@ -720,7 +725,7 @@ def mx_dequantize(codes: Tensor, scales: Tensor, fmt: str, k: int, tensor_scale:
         raise ValueError("mx_dequantize: dtype must be bf16, fp16 or fp32, and k positive")
     code = _mx_check("mx_dequantize", codes, scales, fmt, k, tensor_scale)
     m = codes.shape[0]
-    out = codes.new_empty((m, k), dtype=dtype)
+    out = _matrix(m, k, dtype, dev)
     if m:
         with _on(dev):
             _lib.call("svdq_mx_dequantize", codes.data_ptr(), scales.data_ptr(), code, _ptr(tensor_scale), m, k,
@@ -774,7 +779,7 @@ def mx_gemm(a_codes: Tensor, a_scales: Tensor, a_fmt: str, a_tensor_scale: Optio
     w_code = _mx_check("mx_gemm (weight)", w_codes, w_scales, w_fmt, k, w_tensor_scale)
     m, n = a_codes.shape[0], w_codes.shape[0]
     _mx_gemm_check("mx_gemm", a_fmt, w_fmt, n, bias, out_dtype)
-    out = a_codes.new_empty((m, n), dtype=out_dtype)
+    out = _matrix(m, n, out_dtype, dev)
     if m and n:
         with _on(dev):
             _lib.call("svdq_mx_gemm", a_codes.data_ptr(), a_scales.data_ptr(), a_code, _ptr(a_tensor_scale),
@@ -804,7 +809,7 @@ def mx_linear(x: Tensor, a_fmt: str, a_tensor_scale: Optional[Tensor], w_codes: 
     w_code = _mx_check("mx_linear (weight)", w_codes, w_scales, w_fmt, k, w_tensor_scale)
     n = w_codes.shape[0]
     _mx_gemm_check("mx_linear", a_fmt, w_fmt, n, bias, out_dtype)
-    out = x.new_empty((m, n), dtype=out_dtype)
+    out = _matrix(m, n, out_dtype, dev)
     if m and n:
         ws, n_ws = None, 0
         if m > MX_FUSED_TOKENS:
@@ -840,9 +845,9 @@ def rms_norm_mx(x: Tensor, weight: Optional[Tensor], residual: Optional[Tensor],
         if residual.dtype != x.dtype or residual.shape != x.shape:
             raise ValueError("rms_norm_mx: residual must have x's shape and dtype")
         _, _, ldr = _mx_rows("rms_norm_mx (residual)", residual)
-    codes = x.new_empty((m, mx_k_pad(h)), dtype=torch.float8_e4m3fn)
-    scales = x.new_empty((mx_scales_numel(m, h, "mxfp8"),), dtype=torch.uint8)
-    total = x.new_empty((0,) if residual is None else (m, h))
+    codes = _matrix(m, mx_k_pad(h), torch.float8_e4m3fn, dev)
+    scales = x.new_empty(mx_scales_numel(m, h, "mxfp8"), dtype=torch.uint8)
+    total = x.new_empty(0) if residual is None else _matrix(m, h, x.dtype, dev)
     if m:
         with _on(dev):
             _lib.call("svdq_rms_norm_mx", x.data_ptr(), ld, _ptr(residual), ldr, _ptr(weight), _DT[x.dtype], eps, m, h,
@@ -854,7 +859,7 @@ def rms_norm_mx(x: Tensor, weight: Optional[Tensor], residual: Optional[Tensor],
 @rms_norm_mx.register_fake
 def _(x, weight, residual, eps):
     m, h = x.shape
-    return (_mx_codes_like(x, m, h, "mxfp8"), x.new_empty((mx_scales_numel(m, h, "mxfp8"),), dtype=torch.uint8),
+    return (_mx_codes(m, h, "mxfp8", x.device), x.new_empty((mx_scales_numel(m, h, "mxfp8"),), dtype=torch.uint8),
             x.new_empty((0,) if residual is None else (m, h)))
 
 
