@@ -111,14 +111,25 @@ __device__ __forceinline__ uint32_t e2m1_of(double q) {
   const uint32_t c = (a > 0.25) + (a >= 0.75) + (a > 1.25) + (a >= 1.75) + (a > 2.5) + (a >= 3.5) + (a > 5.0);
   return c | (signbit(q) ? 8u : 0u);
 }
-// An nvfp4 block whose scale or values are near the ends of fp32's range, in 64 bits.
-static __device__ __noinline__ uint2 nvfp4_codes_wide(const float* x, float sf, float g) {
+// An nvfp4 block whose scale or values are near the ends of fp32's range, in 64 bits.  Takes -x.  Rare:
+// one element at a time, picked out of registers, so that it costs the usual path neither
+// registers nor a stack.
+__device__ __forceinline__ uint2 nvfp4_codes_wide(const float (&nx)[16], float sf, float g) {
   const double d = (double)sf * (double)g;
-  uint32_t w[2] = {0u, 0u};
+  uint2 w = make_uint2(0u, 0u);
 #pragma unroll 1
-  for (int i = 0; i < 16; ++i) w[i >> 3] |= e2m1_of((double)x[i] / d) << (4 * (i & 7));
-  return make_uint2(w[0], w[1]);
+  for (int i = 0; i < 16; ++i) {
+    float v = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (j == i) v = -nx[j];
+    const uint32_t c = e2m1_of((double)v / d) << (4 * (i & 7));
+    if (i < 8) w.x |= c;
+    else w.y |= c;
+  }
+  return w;
 }
+
 // What the quotients of an nvfp4 block need, by its scale byte.  A launch has one tensor scale g, so a
 // CTA works this out once per byte.
 struct Nvfp4Unit {
@@ -172,12 +183,7 @@ __device__ __forceinline__ Nvfp4Unit nvfp4_unit(uint32_t byte, float g) {
 __device__ __forceinline__ uint2 nvfp4_codes(const float (&nx)[16], uint32_t amax_bits, uint32_t byte,
                                              const Nvfp4Unit& u, float g) {
   if (byte == 0u || byte == 0x7Fu) return make_uint2(0u, 0u);
-  if (!(__uint_as_float(amax_bits) <= u.limit)) {
-    float v[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = -nx[i];
-    return nvfp4_codes_wide(v, e4m3_value(byte), g);
-  }
+  if (!(__uint_as_float(amax_bits) <= u.limit)) return nvfp4_codes_wide(nx, e4m3_value(byte), g);
   const uint64_t ny = f2_pack(u.ny, u.ny), dd = f2_pack(u.d, u.d);
   float q[16];
 #pragma unroll
@@ -369,6 +375,25 @@ struct CodeWord<kMxfp8> {
   using type = uint4;
 };
 
+// The codes of 16 columns of an mx block from its scale byte.
+template <typename T, int FMT>
+__device__ __forceinline__ typename CodeWord<FMT>::type mx_codes(const T (&x)[16], uint32_t byte) {
+  float v[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = to_float(x[i]);
+  if (byte == 255u) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = 0.0f;
+  }
+  scale_all(v, mx_inverse_scale(byte));
+  if constexpr (FMT == kMxfp4) {
+    return make_uint2(e2m1x8_satfinite(v), e2m1x8_satfinite(v + 8));
+  } else {
+    uint32_t w[4];
+    e4m3_words(v, w);
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
 // The codes of 16 columns (x is overwritten) and their block's scale byte.  An mx block is shared with
 // the neighbouring lane (lane ^ 1), so every lane of the warp takes part.
 template <typename T, int FMT>
@@ -379,29 +404,15 @@ __device__ __forceinline__ typename CodeWord<FMT>::type encode_chunk(T (&x)[16],
     constexpr uint32_t kSigns = sizeof(T) == 2 ? 0x80008000u : 0x80000000u;
 #pragma unroll
     for (int i = 0; i < (int)sizeof(T) * 4; ++i) reinterpret_cast<uint32_t*>(x)[i] ^= kSigns;
-  } else {
-    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-  }
-  float v[16];
+    float v[16];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) v[i] = to_float(x[i]);
-  if constexpr (FMT == kNvfp4) {
+    for (int i = 0; i < 16; ++i) v[i] = to_float(x[i]);
     byte = nvfp4_scale_byte(amax, g);
     return nvfp4_codes(v, amax, byte, units[byte], g);
   } else {
+    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
     byte = mx_scale_byte<FMT>(amax);
-    if (byte == 255u) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = 0.0f;
-    }
-    scale_all(v, mx_inverse_scale(byte));
-    if constexpr (FMT == kMxfp4) {
-      return make_uint2(e2m1x8_satfinite(v), e2m1x8_satfinite(v + 8));
-    } else {
-      uint32_t w[4];
-      e4m3_words(v, w);
-      return make_uint4(w[0], w[1], w[2], w[3]);
-    }
+    return mx_codes<T, FMT>(x, byte);
   }
 }
 // The four scale bytes of a word, from the 4 (nvfp4) or 8 (mx) neighbouring lanes that have them.

@@ -5,7 +5,6 @@ namespace svdq {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kCtasPerSm = 4;  // of the quantisation to nvfp4, whose CTAs stay for a whole launch
 
 // Quotient and remainder by a divisor that is fixed for a launch: floor(n / d) = (n * mul) >> 32 >>
 // shift with mul = ceil(2^(32 + shift) / d), exact for n < 2^31 (T. Granlund, P. Montgomery,
@@ -23,48 +22,47 @@ __device__ __forceinline__ uint32_t div_by(const FastDiv& f, uint32_t n) {
   return f.d == 1 ? n : __umulhi(n, f.mul) >> (f.shift - 1);
 }
 
-// Chunks of 16 elements per thread: 64 bytes in flight.
+// Chunks of 16 elements that a thread reads back: 64 bytes written.
 template <typename T>
 __host__ __device__ constexpr int unroll_of() { return sizeof(T) == 2 ? 2 : 1; }
+// Columns that a thread quantises: 64 bytes read.
+template <typename T>
+__host__ __device__ constexpr int columns_of() { return 64 / (int)sizeof(T); }
+
 struct QuantArgs {
   const void* x;
   int64_t ldx;
   int M, K;
-  int rows;            // rows with scales: M rounded up to 128
-  uint32_t chunks;     // rows * chunks per row
-  FastDiv per_row;     // 16-column chunks per row, K_pad / 16
+  uint32_t chunks;     // chunks of all rows with scales (M rounded up to 128)
+  FastDiv per_row;     // chunks per row
   bool vec;
   const float* tensor_scale;
   uint8_t* codes;
   uint8_t* scales;
 };
 
-// One thread quantises 16 columns of a row: a whole nvfp4 block, or half an mx block whose other
-// half is the neighbouring lane's.  Bound by HBM: 2 bytes read and 0.56 written per element from
-// bf16 to nvfp4.  The four scale bytes of a 32-bit word of the tile layout come from 4 (nvfp4) or 8
-// (mx) neighbouring lanes and leave as one store.
+// A thread quantises 64 bytes of a row: 32 columns of a 16-bit type, which are two nvfp4 blocks or one mx
+// block, or 16 columns in fp32, one nvfp4 block or half an mx block whose other half is the
+// neighbouring lane's.  HBM moves 2 bytes in and 0.5 out per element from bf16 to a 4-bit
+// format; the instructions for them are nearly as much work, so what is done once per thread is shared
+// by as many columns as stay in registers (16 columns a thread: 13.0 us to mxfp4, 32: 11.6, which is 5.8
+// TB/s; to nvfp4 the instructions bound it, 18 us or 3.8 TB/s, all at 4352 x 6144 from bf16).  The four scale bytes of a 32-bit word of the tile
+// layout come from 2 to 8 neighbouring lanes and leave as one store.
+//
+// A CTA takes kThreads neighbouring chunks.  From fp32 to nvfp4 it stays for a share of the launch's
+// chunks, with the loads of the next ones issued before the present ones are worked on, because its
+// units cost as much as half a step (4352 x 6144: 21.8 us against 25.5); the others run faster one
+// step to a CTA (from bf16 to nvfp4 18.1 us against 20.4, to mxfp4 11.6).  VEC: rows on 32-byte
+// boundaries and K a multiple of 16.
 template <typename T, int FMT>
-__device__ __forceinline__ void quantize_chunk(const QuantArgs& a, T (&x)[16], uint32_t id, int row, int chunk,
-                                               bool live, float g, const Nvfp4Unit* units) {
-  using Codes = typename CodeWord<FMT>::type;
-  uint32_t byte;
-  const Codes codes = encode_chunk<T, FMT>(x, g, units, byte);
-  if (live)
-    reinterpret_cast<Codes*>(a.codes + (size_t)row * mx_row_bytes(FMT, (int)a.per_row.d * 16))[chunk] = codes;
-  constexpr int kLanes = FMT == kNvfp4 ? 4 : 8;  // per word of scales
-  const uint32_t word = scale_word<FMT>(live ? byte : 0u);
-  if (id < a.chunks && (threadIdx.x & 31) % kLanes == 0)
-    *reinterpret_cast<uint32_t*>(a.scales + mx_scale_word(row, chunk / kLanes, (int)a.per_row.d / kLanes)) = word;
-}
+__host__ __device__ constexpr bool stays() { return FMT == kNvfp4 && sizeof(T) == 4; }
+constexpr int kStayCtas = 3;  // per SM: 256 threads of up to 80 registers
 
-// A CTA takes kThreads * kUnroll neighbouring chunks at a time.  For nvfp4 it stays for a share of
-// the launch's chunks, since it works out its units first, with the loads of the next chunks issued
-// before the present ones are worked on; the mx formats have nothing to share and run faster one step to
-// a CTA (4352 x 16384 bf16 to mxfp4: 31 us against 36).  VEC: rows on 32-byte boundaries and K a
-// multiple of 16.
 template <typename T, int FMT, bool VEC>
 __global__ void __launch_bounds__(kThreads) mx_quantize_kernel(const QuantArgs a) {
-  constexpr int kUnroll = unroll_of<T>();
+  constexpr int C = columns_of<T>(), kPieces = C / 16;
+  constexpr int kRowUnits = 128 / C;  // chunks per 128 columns
+  using Codes = typename CodeWord<FMT>::type;
   __shared__ __align__(16) Nvfp4Unit units[FMT == kNvfp4 ? 128 : 1];
   pdl_wait();
   pdl_trigger();
@@ -73,54 +71,96 @@ __global__ void __launch_bounds__(kThreads) mx_quantize_kernel(const QuantArgs a
     int row, chunk;
     bool live;
   };
-  auto place = [&](uint32_t step, int u) {
+  auto place = [&](uint32_t step) {
     Place p;
-    p.id = (step * kUnroll + u) * kThreads + threadIdx.x;
+    p.id = step * kThreads + threadIdx.x;
     const uint32_t r = div_by(a.per_row, p.id);
     p.row = (int)r;
     p.chunk = (int)(p.id - r * a.per_row.d);
     p.live = p.id < a.chunks && p.row < a.M;
     return p;
   };
-  auto load = [&](const Place& p, T (&x)[16]) {
+  auto load = [&](const Place& p, T (&x)[kPieces][16]) {
     const T* src = static_cast<const T*>(a.x) + (p.live ? (size_t)p.row * a.ldx : 0);
-    const int c = p.live ? p.chunk * 16 : a.K;
+    const int c = p.live ? p.chunk * C : a.K;
     if constexpr (VEC) {
-      if (c < a.K) {
-        load_vec(src + c, x);
-      } else {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = from_float<T>(0.0f);
+      for (int h = 0; h < kPieces; ++h) {
+        if (c + 16 * h < a.K) {
+          load_vec(src + c + 16 * h, x[h]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x[h][i] = from_float<T>(0.0f);
+        }
       }
     } else {
-      load_shifted(src, c, a.K, x);
+      load_shifted(src, c, a.K, reinterpret_cast<T(&)[C]>(x));
     }
   };
-  const uint32_t steps = (a.chunks + kThreads * kUnroll - 1) / (kThreads * kUnroll);
-  alignas(32) T x[kUnroll][16];
-#pragma unroll
-  for (int u = 0; u < kUnroll; ++u) load(place(blockIdx.x, u), x[u]);
+  const uint32_t steps = (a.chunks + kThreads - 1) / kThreads;
+  alignas(32) T x[kPieces][16];
+  Place at = place(blockIdx.x);
+  load(at, x);
   const float g = a.tensor_scale ? *a.tensor_scale : 1.0f;
   if constexpr (FMT == kNvfp4) {
     if (threadIdx.x < 128) units[threadIdx.x] = nvfp4_unit<significant_bits<T>()>(threadIdx.x, g);
     __syncthreads();
   }
   for (uint32_t step = blockIdx.x; step < steps; step += gridDim.x) {
-    alignas(32) T next[kUnroll][16];
-    if (FMT == kNvfp4 && step + gridDim.x < steps) {
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) load(place(step + gridDim.x, u), next[u]);
+    alignas(32) T next[kPieces][16];
+    Place then{};
+    if (stays<T, FMT>() && step + gridDim.x < steps) {
+      then = place(step + gridDim.x);
+      load(then, next);
     }
+    Codes codes[kPieces];
+    uint32_t word;
+    if constexpr (FMT == kNvfp4) {
+      uint32_t bytes = 0;
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const Place p = place(step, u);
-      quantize_chunk<T, FMT>(a, x[u], p.id, p.row, p.chunk, p.live, g, units);
+      for (int h = 0; h < kPieces; ++h) {
+        uint32_t byte;
+        codes[h] = encode_chunk<T, FMT>(x[h], g, units, byte);
+        bytes |= byte << (8 * h);
+      }
+      if (!at.live) bytes = 0;
+      word = bytes << (8 * kPieces * (threadIdx.x & (4 / kPieces - 1)));
+      word |= __shfl_xor_sync(0xffffffffu, word, 1);
+      if (kPieces == 1) word |= __shfl_xor_sync(0xffffffffu, word, 2);
+    } else {
+      uint32_t amax = 0;
+#pragma unroll
+      for (int h = 0; h < kPieces; ++h) amax = max(amax, amax_bits_of(x[h]));
+      if (kPieces == 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+      const uint32_t byte = mx_scale_byte<FMT>(amax);
+#pragma unroll
+      for (int h = 0; h < kPieces; ++h) codes[h] = mx_codes<T, FMT>(x[h], byte);
+      constexpr int L = 2 / kPieces;  // lanes per block
+      word = (at.live ? byte : 0u) << (8 * ((threadIdx.x / L) & 3));
+      word |= __shfl_xor_sync(0xffffffffu, word, L);
+      word |= __shfl_xor_sync(0xffffffffu, word, 2 * L);
     }
+    if (at.live) {
+      Codes* to = reinterpret_cast<Codes*>(a.codes + (size_t)at.row * mx_row_bytes(FMT, (int)a.per_row.d * C)) +
+                  at.chunk * kPieces;
+      if constexpr (kPieces == 2 && FMT != kMxfp8) {
+        *reinterpret_cast<uint4*>(to) = make_uint4(codes[0].x, codes[0].y, codes[1].x, codes[1].y);
+      } else {
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
+        for (int h = 0; h < kPieces; ++h) to[h] = codes[h];
+      }
+    }
+    constexpr int kLanes = (FMT == kNvfp4 ? 64 : 128) / C;  // lanes per word
+    if (at.id < a.chunks && (threadIdx.x & (kLanes - 1)) == 0) {
+      const int words = (int)a.per_row.d / kRowUnits * (FMT == kNvfp4 ? 2 : 1);
+      *reinterpret_cast<uint32_t*>(a.scales + mx_scale_word(at.row, at.chunk / kLanes, words)) = word;
+    }
+    if (!stays<T, FMT>()) break;
+    at = then;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) x[u][i] = next[u][i];
-    if (FMT != kNvfp4) break;
+    for (int h = 0; h < kPieces; ++h)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[h][i] = next[h][i];
   }
 }
 
@@ -223,11 +263,11 @@ __global__ void mx_tensor_scale_kernel(float* out) {
   *out = amax == 0.0f ? 1.0f : amax / 2688.0f;
 }
 
-// chunks and per_row of an [M, K] matrix padded to K_pad columns; false where a launch cannot hold it
-bool chunk_grid(int rows, int K, uint32_t* chunks, FastDiv* per_row) {
-  const uint32_t per = (uint32_t)mx_k_pad(K) / 16;
+// chunks and per_row of a matrix of `rows` rows in chunks of C columns; false where a launch cannot hold it
+bool chunk_grid(int rows, int K, int C, uint32_t* chunks, FastDiv* per_row) {
+  const uint32_t per = (uint32_t)mx_k_pad(K) / C;
   const uint64_t n = (uint64_t)rows * per;
-  if (n >= (1ull << 31)) return false;
+  if ((uint64_t)rows * mx_k_pad(K) >= (1ull << 35)) return false;
   *chunks = (uint32_t)n;
   *per_row = fast_div(per);
   return true;
@@ -235,9 +275,8 @@ bool chunk_grid(int rows, int K, uint32_t* chunks, FastDiv* per_row) {
 
 template <typename T, bool VEC>
 int launch_quantize(int fmt, const QuantArgs& a, cudaStream_t stream) {
-  const uint32_t per = kThreads * unroll_of<T>(), most = (uint32_t)num_sms() * kCtasPerSm;
-  const uint32_t steps = (a.chunks + per - 1) / per;
-  const dim3 grid(fmt == kNvfp4 && steps > most ? most : steps), block(kThreads);
+  const uint32_t steps = (a.chunks + kThreads - 1) / kThreads, most = (uint32_t)num_sms() * kStayCtas;
+  const dim3 grid(fmt == kNvfp4 && stays<T, kNvfp4>() && steps > most ? most : steps), block(kThreads);
   const char* what = "svdq_mx_quantize launch";
   if (fmt == kNvfp4) return launch_pdl(what, mx_quantize_kernel<T, kNvfp4, VEC>, grid, block, 0, stream, 1, a);
   if (fmt == kMxfp4) return launch_pdl(what, mx_quantize_kernel<T, kMxfp4, VEC>, grid, block, 0, stream, 1, a);
@@ -274,13 +313,12 @@ extern "C" int svdq_mx_quantize(const void* x, int64_t ldx, int dtype, int M, in
   SVDQ_REQUIRE(((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(scales)) & 15u) == 0,
                "svdq_mx_quantize: codes and scales must be 16-byte aligned");
   QuantArgs a{};
-  if (M > (1 << 30) || K > (1 << 30) || !chunk_grid(mx_rows_pad(M), K, &a.chunks, &a.per_row))
+  if (M > (1 << 30) || K > (1 << 30) || !chunk_grid(mx_rows_pad(M), K, 64 / dtype_bytes(dtype), &a.chunks, &a.per_row))
     return set_error(SVDQ_ERR_UNSUPPORTED, "svdq_mx_quantize: more than 2^35 padded elements");
   a.x = x;
   a.ldx = ldx;
   a.M = M;
   a.K = K;
-  a.rows = mx_rows_pad(M);
   a.vec = K % 16 == 0 && rows_aligned(x, ldx, dtype_bytes(dtype), 32);
   a.tensor_scale = tensor_scale;
   a.codes = static_cast<uint8_t*>(codes);
@@ -302,7 +340,7 @@ extern "C" int svdq_mx_dequantize(const void* codes, const void* scales, int for
   SVDQ_REQUIRE(((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(scales)) & 15u) == 0,
                "svdq_mx_dequantize: codes and scales must be 16-byte aligned");
   ReadArgs a{};
-  if (M > (1 << 30) || K > (1 << 30) || !chunk_grid(M, K, &a.chunks, &a.per_row))
+  if (M > (1 << 30) || K > (1 << 30) || !chunk_grid(M, K, 16, &a.chunks, &a.per_row))
     return set_error(SVDQ_ERR_UNSUPPORTED, "svdq_mx_dequantize: more than 2^35 padded elements");
   a.codes = static_cast<const uint8_t*>(codes);
   a.scales = static_cast<const uint8_t*>(scales);
@@ -327,7 +365,7 @@ extern "C" int svdq_mx_tensor_scale(const void* x, int64_t ldx, int dtype, int M
   if (st) return st;
   uint32_t chunks = 0;
   FastDiv per_row{};
-  if (M > (1 << 30) || K > (1 << 30) || !chunk_grid(M, K, &chunks, &per_row))
+  if (M > (1 << 30) || K > (1 << 30) || !chunk_grid(M, K, 16, &chunks, &per_row))
     return set_error(SVDQ_ERR_UNSUPPORTED, "svdq_mx_tensor_scale: more than 2^35 padded elements");
   if (chunks > 0) {
     const bool vec = K % 16 == 0 && rows_aligned(x, ldx, dtype_bytes(dtype), 32);
