@@ -161,7 +161,8 @@ int launch_norm(const NormArgs& a, cudaStream_t stream) {
   const int chunks = a.h_pad / C;
   if (chunks <= 128) return launch_pdl(what, rms_norm_mx_kernel<T, 128, 1, VEC>, grid, dim3(128), 0, stream, 1, a);
   if (chunks <= 256) return launch_pdl(what, rms_norm_mx_kernel<T, 128, 2, VEC>, grid, dim3(128), 0, stream, 1, a);
-  if (chunks <= 384) return launch_pdl(what, rms_norm_mx_kernel<T, 128, 3, VEC>, grid, dim3(128), 0, stream, 1, a);
+  if (chunks <= 384 && sizeof(T) == 2)  // three passes of fp32 do not fit the registers
+    return launch_pdl(what, rms_norm_mx_kernel<T, 128, 3, VEC>, grid, dim3(128), 0, stream, 1, a);
   if (chunks <= 512) return launch_pdl(what, rms_norm_mx_kernel<T, 256, 2, VEC>, grid, dim3(256), 0, stream, 1, a);
   if (chunks <= 768) return launch_pdl(what, rms_norm_mx_kernel<T, 256, 3, VEC>, grid, dim3(256), 0, stream, 1, a);
   if (chunks <= 1024) return launch_pdl(what, rms_norm_mx_kernel<T, 256, 4, VEC>, grid, dim3(256), 0, stream, 1, a);

@@ -429,6 +429,31 @@ def test_few_tokens_quantised_by_the_product(act, w_fmt, dtype, m, n, k, cut):
     no_device_error()
 
 
+def test_registered_ops():
+    """The operators as torch custom ops: the same results, shapes under fake tensors, and a compiled call."""
+    from krea2_svdquant_b200 import ops
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    M, e, o = ms(), ops.eager, torch.ops.svdq_b200
+    x, w = data(20, 300, torch.bfloat16), data(70, 300, seed=1)
+    wq = M.quantize(w, "mxfp4")
+    calls = {"mx_quantize": (x, "mxfp8", None), "mx_tensor_scale": (x,), "rms_norm_mx": (x, None, x, 1e-6),
+             "mx_dequantize": (wq.codes, wq.scales, "mxfp4", 300, None, torch.float16),
+             "mx_linear": (x, "mxfp8", None, wq.codes, wq.scales, "mxfp4", None, None, torch.bfloat16)}
+    a = M.quantize(x, "mxfp4")
+    calls["mx_gemm"] = (a.codes, a.scales, "mxfp4", None, wq.codes, wq.scales, "mxfp4", None, 300, None, torch.float32)
+    for name, args in calls.items():
+        got, want = getattr(o, name)(*args), getattr(e, name)(*args)
+        got, want = (r if isinstance(r, (list, tuple)) else (r,) for r in (got, want))
+        with FakeTensorMode() as mode:
+            fake = getattr(o, name)(*[mode.from_tensor(v) if isinstance(v, torch.Tensor) else v for v in args])
+        fake = fake if isinstance(fake, (list, tuple)) else (fake,)
+        for g, r, f in zip(got, want, fake, strict=True):
+            assert torch.equal(g.view(torch.uint8), r.view(torch.uint8))
+            assert (f.shape, f.dtype) == (r.shape, r.dtype)
+    run = lambda v: M.linear(M.rms_norm(v, residual=v)[0], wq) + M.linear(v, wq, act="mxfp8")
+    assert torch.equal(torch.compile(run, fullgraph=True, backend="aot_eager")(x), run(x))
+
+
 def test_empty_batches():
     M = ms()
     w = M.quantize(data(64, 128), "nvfp4")
