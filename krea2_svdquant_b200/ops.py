@@ -37,26 +37,23 @@ def _stream(dev: torch.device):
     return ctypes.c_void_p(_raw_stream(dev))
 
 
-class _Here:
-    """A ``with`` block that changes nothing."""
-
-    def __enter__(self):
-        return self
-
-    def __exit__(self, *exc):
-        return False
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
-_HERE = _Here()
-
-
-def _on(dev: torch.device):
-    """Makes ``dev`` the current device for a launch: a stream of one device takes no launch while
-    another device is current.  (``torch.cuda.device`` costs several us, so only where it changes
-    something.)"""
-    if dev.index is None or dev.index == torch._C._cuda_getDevice():
-        return _HERE
-    return torch.cuda.device(dev)
+def _launch(dev: torch.device, name: str, *args) -> None:
+    """Calls an entry point on ``dev``'s current stream (its last argument), with ``dev`` current: a
+    stream of one device takes no launch while another is current.  (``torch.cuda.device`` costs
+    several us, so only where it changes something.)"""
+    fn = getattr(_lib.lib(), name)
+    i = dev.index
+    if i is None or i == _current_device():
+        st = fn(*args, _raw_stream(dev) if _current_stream is None or i is None else _current_stream(i))
+    else:
+        with torch.cuda.device(dev):
+            st = fn(*args, _raw_stream(dev))
+    if st:
+        _lib.check(st)
 
 
 def _need_cuda(name: str, *ts: Optional[Tensor]) -> None:
@@ -674,9 +671,11 @@ def _mx_rows(who: str, x: Tensor) -> tuple[int, int, int]:
     if x.dim() != 2 or x.dtype not in _DT:
         raise ValueError(f"{who}: expected a 2-D bf16, fp16 or fp32 tensor, got {x.dtype} {tuple(x.shape)}")
     m, k = x.shape
-    if k == 0 or (k > 1 and x.stride(1) != 1):
+    ld, step = x.stride()
+    if k == 0 or (k > 1 and step != 1):
         raise ValueError(f"{who}: rows must have columns and unit column stride")
-    ld = x.stride(0) if m > 1 else k  # the stride of a single row means nothing
+    if m <= 1:
+        ld = k  # the stride of a single row means nothing
     if ld < k:
         raise ValueError(f"{who}: rows must not overlap (row stride {ld} of {k} columns)")
     return m, k, ld
@@ -704,9 +703,8 @@ def mx_quantize(x: Tensor, fmt: str, tensor_scale: Optional[Tensor]) -> tuple[Te
     codes = _mx_codes(m, k, fmt, dev)
     scales = x.new_empty(mx_scales_numel(m, k, fmt), dtype=torch.uint8)
     if m:
-        with _on(dev):
-            _lib.call("svdq_mx_quantize", x.data_ptr(), ld, _DT[x.dtype], m, k, code, _ptr(tensor_scale),
-                      codes.data_ptr(), scales.data_ptr(), _raw_stream(dev))
+        _launch(dev, "svdq_mx_quantize", x.data_ptr(), ld, _DT[x.dtype], m, k, code, _ptr(tensor_scale),
+                codes.data_ptr(), scales.data_ptr())
     return codes, scales
 
 
@@ -727,9 +725,8 @@ def mx_dequantize(codes: Tensor, scales: Tensor, fmt: str, k: int, tensor_scale:
     m = codes.shape[0]
     out = _matrix(m, k, dtype, dev)
     if m:
-        with _on(dev):
-            _lib.call("svdq_mx_dequantize", codes.data_ptr(), scales.data_ptr(), code, _ptr(tensor_scale), m, k,
-                      out.data_ptr(), k, _DT[dtype], _raw_stream(dev))
+        _launch(dev, "svdq_mx_dequantize", codes.data_ptr(), scales.data_ptr(), code, _ptr(tensor_scale), m, k,
+                out.data_ptr(), k, _DT[dtype])
     return out
 
 
@@ -744,8 +741,7 @@ def mx_tensor_scale(x: Tensor) -> Tensor:
     dev = _mx_device("mx_tensor_scale", x)
     m, k, ld = _mx_rows("mx_tensor_scale", x)
     out = x.new_empty((1,), dtype=torch.float32)
-    with _on(dev):
-        _lib.call("svdq_mx_tensor_scale", _p(x), ld, _DT[x.dtype], m, k, out.data_ptr(), _raw_stream(dev))
+    _launch(dev, "svdq_mx_tensor_scale", _p(x), ld, _DT[x.dtype], m, k, out.data_ptr())
     return out
 
 
@@ -781,10 +777,9 @@ def mx_gemm(a_codes: Tensor, a_scales: Tensor, a_fmt: str, a_tensor_scale: Optio
     _mx_gemm_check("mx_gemm", a_fmt, w_fmt, n, bias, out_dtype)
     out = _matrix(m, n, out_dtype, dev)
     if m and n:
-        with _on(dev):
-            _lib.call("svdq_mx_gemm", a_codes.data_ptr(), a_scales.data_ptr(), a_code, _ptr(a_tensor_scale),
-                      w_codes.data_ptr(), w_scales.data_ptr(), w_code, _ptr(w_tensor_scale), _ptr(bias),
-                      out.data_ptr(), _DT[out_dtype], n, m, n, k, _raw_stream(dev))
+        _launch(dev, "svdq_mx_gemm", a_codes.data_ptr(), a_scales.data_ptr(), a_code, _ptr(a_tensor_scale),
+                w_codes.data_ptr(), w_scales.data_ptr(), w_code, _ptr(w_tensor_scale), _ptr(bias),
+                out.data_ptr(), _DT[out_dtype], n, m, n, k)
     return out
 
 
@@ -816,10 +811,9 @@ def mx_linear(x: Tensor, a_fmt: str, a_tensor_scale: Optional[Tensor], w_codes: 
             codes = m * mx_k_pad(k) // (1 if a_fmt == "mxfp8" else 2)
             n_ws = (codes + 255) // 256 * 256 + mx_scales_numel(m, k, a_fmt)
             ws = x.new_empty(n_ws, dtype=torch.uint8)
-        with _on(dev):
-            _lib.call("svdq_mx_linear", x.data_ptr(), ld, _DT[x.dtype], a_code, _ptr(a_tensor_scale),
-                      w_codes.data_ptr(), w_scales.data_ptr(), w_code, _ptr(w_tensor_scale), _ptr(bias),
-                      out.data_ptr(), _DT[out_dtype], n, m, n, k, _ptr(ws), n_ws, _raw_stream(dev))
+        _launch(dev, "svdq_mx_linear", x.data_ptr(), ld, _DT[x.dtype], a_code, _ptr(a_tensor_scale),
+                w_codes.data_ptr(), w_scales.data_ptr(), w_code, _ptr(w_tensor_scale), _ptr(bias),
+                out.data_ptr(), _DT[out_dtype], n, m, n, k, _ptr(ws), n_ws)
     return out
 
 
@@ -849,10 +843,8 @@ def rms_norm_mx(x: Tensor, weight: Optional[Tensor], residual: Optional[Tensor],
     scales = x.new_empty(mx_scales_numel(m, h, "mxfp8"), dtype=torch.uint8)
     total = x.new_empty(0) if residual is None else _matrix(m, h, x.dtype, dev)
     if m:
-        with _on(dev):
-            _lib.call("svdq_rms_norm_mx", x.data_ptr(), ld, _ptr(residual), ldr, _ptr(weight), _DT[x.dtype], eps, m, h,
-                      codes.data_ptr(), scales.data_ptr(), None if residual is None else total.data_ptr(), h,
-                      _raw_stream(dev))
+        _launch(dev, "svdq_rms_norm_mx", x.data_ptr(), ld, _ptr(residual), ldr, _ptr(weight), _DT[x.dtype], eps, m, h,
+                codes.data_ptr(), scales.data_ptr(), None if residual is None else total.data_ptr(), h)
     return codes, scales, total
 
 
