@@ -429,6 +429,7 @@ __device__ __forceinline__ uint32_t scale_word(uint32_t byte) {
 inline bool rows_aligned(const void* p, int64_t ld, int elem_bytes, int align) {
   return reinterpret_cast<uintptr_t>(p) % align == 0 && (ld * elem_bytes) % align == 0;
 }
+inline bool element_aligned(const void* p, int elem_bytes) { return reinterpret_cast<uintptr_t>(p) % elem_bytes == 0; }
 inline int dtype_bytes(int dtype) { return dtype == SVDQ_FP32 ? 4 : 2; }
 inline bool dtype_ok(int dtype) { return dtype == SVDQ_BF16 || dtype == SVDQ_FP16 || dtype == SVDQ_FP32; }
 inline bool mx_format_ok(int fmt) { return fmt == kNvfp4 || fmt == kMxfp4 || fmt == kMxfp8; }

@@ -490,9 +490,9 @@ int mx_product(MxGemm& g, int K) {
   SVDQ_REQUIRE(((reinterpret_cast<uintptr_t>(g.a_codes) | reinterpret_cast<uintptr_t>(g.a_scales) |
                  reinterpret_cast<uintptr_t>(g.w_codes) | reinterpret_cast<uintptr_t>(g.w_scales)) & 31u) == 0,
                "svdq_mx_gemm: codes and scales must be 32-byte aligned");
-  SVDQ_REQUIRE((reinterpret_cast<uintptr_t>(g.o.out) % dtype_bytes(g.o.out_dtype)) == 0 &&
-                   (reinterpret_cast<uintptr_t>(g.o.bias) & 1u) == 0,
-               "svdq_mx_gemm: out and bias must be aligned to their elements");
+  SVDQ_REQUIRE(element_aligned(g.o.out, dtype_bytes(g.o.out_dtype)) && element_aligned(g.o.bias, 2) &&
+                   element_aligned(g.o.a_scale, 4) && element_aligned(g.o.w_scale, 4),
+               "svdq_mx_gemm: out, bias and tensor scales must be aligned to their elements");
   if (M > (1 << 24) || N > (1 << 24) || K > (1 << 28))
     return set_error(SVDQ_ERR_UNSUPPORTED, "svdq_mx_gemm: M and N up to 2^24, K up to 2^28");
   g.mode = g.a_fmt == kNvfp4 ? kModeNvfp4 : g.a_fmt == kMxfp4 ? kModeMxfp4 : kModeW4A8;
@@ -542,7 +542,7 @@ extern "C" int svdq_mx_linear(const void* x, int64_t ldx, int dtype, int a_forma
   SVDQ_REQUIRE(dtype_ok(dtype), "svdq_mx_linear: x must be bf16, fp16 or fp32");
   SVDQ_REQUIRE(M >= 0 && K > 0 && ldx >= K, "svdq_mx_linear: bad M/K/ldx");
   SVDQ_REQUIRE(x || M == 0, "svdq_mx_linear: null pointer");
-  SVDQ_REQUIRE((reinterpret_cast<uintptr_t>(x) % dtype_bytes(dtype)) == 0, "svdq_mx_linear: x must be aligned to its elements");
+  SVDQ_REQUIRE(element_aligned(x, dtype_bytes(dtype)), "svdq_mx_linear: x must be aligned to its elements");
   MxGemm g{};
   g.a_fmt = a_format;
   g.w_codes = w_codes;

@@ -186,9 +186,12 @@ extern "C" int svdq_rms_norm_mx(const void* x, int64_t ldx, const void* residual
   SVDQ_REQUIRE(x && codes && scales, "svdq_rms_norm_mx: null pointer");
   SVDQ_REQUIRE(((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(scales)) & 15u) == 0,
                "svdq_rms_norm_mx: codes and scales must be 16-byte aligned");
+  const int elem = dtype_bytes(dtype);
+  SVDQ_REQUIRE(element_aligned(x, elem) && element_aligned(residual, elem) && element_aligned(weight, elem) &&
+                   element_aligned(sum, elem),
+               "svdq_rms_norm_mx: x, residual, weight and sum must be aligned to their elements");
   if (M > (1 << 30) || H > (1 << 30)) return set_error(SVDQ_ERR_UNSUPPORTED, "svdq_rms_norm_mx: matrix too large");
   NormArgs a{};
-  const int eb = dtype_bytes(dtype);
   a.x = x;
   a.ldx = ldx;
   a.residual = residual;
@@ -199,10 +202,9 @@ extern "C" int svdq_rms_norm_mx(const void* x, int64_t ldx, const void* residual
   a.M = M;
   a.H = H;
   a.h_pad = mx_k_pad(H);
-  const int al = 32;
-  const bool vec = H % (32 / eb) == 0 && rows_aligned(x, ldx, eb, al) &&
-                   (!residual || (rows_aligned(residual, ldr, eb, al) && rows_aligned(sum, lds, eb, al))) &&
-                   reinterpret_cast<uintptr_t>(weight) % al == 0;
+  const bool vec = H % (32 / elem) == 0 && rows_aligned(x, ldx, elem, 32) &&
+                   (!residual || (rows_aligned(residual, ldr, elem, 32) && rows_aligned(sum, lds, elem, 32))) &&
+                   reinterpret_cast<uintptr_t>(weight) % 32 == 0;
   a.codes = static_cast<uint8_t*>(codes);
   a.scales = static_cast<uint8_t*>(scales);
   a.sum = sum;

@@ -312,6 +312,8 @@ extern "C" int svdq_mx_quantize(const void* x, int64_t ldx, int dtype, int M, in
   SVDQ_REQUIRE(x && codes && scales, "svdq_mx_quantize: null pointer");
   SVDQ_REQUIRE(((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(scales)) & 15u) == 0,
                "svdq_mx_quantize: codes and scales must be 16-byte aligned");
+  SVDQ_REQUIRE(element_aligned(x, dtype_bytes(dtype)) && element_aligned(tensor_scale, 4),
+               "svdq_mx_quantize: x and tensor_scale must be aligned to their elements");
   QuantArgs a{};
   if (M > (1 << 30) || K > (1 << 30) || !chunk_grid(mx_rows_pad(M), K, 64 / dtype_bytes(dtype), &a.chunks, &a.per_row))
     return set_error(SVDQ_ERR_UNSUPPORTED, "svdq_mx_quantize: more than 2^35 padded elements");
@@ -339,6 +341,8 @@ extern "C" int svdq_mx_dequantize(const void* codes, const void* scales, int for
   SVDQ_REQUIRE(codes && scales && out, "svdq_mx_dequantize: null pointer");
   SVDQ_REQUIRE(((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(scales)) & 15u) == 0,
                "svdq_mx_dequantize: codes and scales must be 16-byte aligned");
+  SVDQ_REQUIRE(element_aligned(out, dtype_bytes(dtype)) && element_aligned(tensor_scale, 4),
+               "svdq_mx_dequantize: out and tensor_scale must be aligned to their elements");
   ReadArgs a{};
   if (M > (1 << 30) || K > (1 << 30) || !chunk_grid(M, K, 16, &a.chunks, &a.per_row))
     return set_error(SVDQ_ERR_UNSUPPORTED, "svdq_mx_dequantize: more than 2^35 padded elements");
@@ -361,6 +365,8 @@ extern "C" int svdq_mx_tensor_scale(const void* x, int64_t ldx, int dtype, int M
   SVDQ_REQUIRE(dtype_ok(dtype), "svdq_mx_tensor_scale: x must be bf16, fp16 or fp32");
   SVDQ_REQUIRE(M >= 0 && K > 0 && ldx >= K, "svdq_mx_tensor_scale: bad M/K/ldx");
   SVDQ_REQUIRE(out && (x || M == 0), "svdq_mx_tensor_scale: null pointer");
+  SVDQ_REQUIRE(element_aligned(x, dtype_bytes(dtype)) && element_aligned(out, 4),
+               "svdq_mx_tensor_scale: x and out must be aligned to their elements");
   int st = check_cuda(cudaMemsetAsync(out, 0, sizeof(float), stream), "svdq_mx_tensor_scale: clear");
   if (st) return st;
   uint32_t chunks = 0;

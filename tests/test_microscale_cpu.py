@@ -125,8 +125,16 @@ def test_c_abi_refusals():
     assert L.svdq_mx_quantize(p, 63, 0, 4, 64, 0, None, p, p, None) == 1
     assert L.svdq_mx_quantize(p, 64, 0, 4, 64, 1, p, p, p, None) == 1 and "tensor scale" in last()
     assert L.svdq_mx_quantize(p, 64, 0, 4, 64, 0, None, ctypes.c_void_p(4100), p, None) == 1 and "aligned" in last()
+    assert L.svdq_mx_quantize(ctypes.c_void_p(4097), 64, 0, 4, 64, 0, None, p, p, None) == 1 and "elements" in last()
+    assert L.svdq_mx_quantize(p, 64, 0, 4, 64, 0, ctypes.c_void_p(4098), p, p, None) == 1
+    assert L.svdq_mx_dequantize(p, p, 0, None, 4, 64, ctypes.c_void_p(4098), 64, 2, None) == 1
+    assert L.svdq_mx_tensor_scale(ctypes.c_void_p(4098), 64, 2, 4, 64, p, None) == 1
     assert L.svdq_mx_quantize(None, 64, 0, 4, 64, 0, None, p, p, None) == 1
     assert L.svdq_mx_quantize(p, 1 << 20, 0, 1 << 20, 1 << 20, 0, None, p, p, None) == 2
+    assert L.svdq_mx_quantize(ctypes.c_void_p(4097), 64, 0, 4, 64, 0, None, p, p, None) == 1 and "elements" in last()
+    assert L.svdq_mx_quantize(p, 64, 0, 4, 64, 0, ctypes.c_void_p(4098), p, p, None) == 1
+    assert L.svdq_mx_dequantize(p, p, 0, None, 4, 64, ctypes.c_void_p(4098), 64, 2, None) == 1
+    assert L.svdq_mx_tensor_scale(ctypes.c_void_p(4098), 64, 2, 4, 64, p, None) == 1
     assert L.svdq_mx_quantize(None, 64, 0, 0, 64, 0, None, None, None, None) == 0  # no rows: nothing to do
     assert L.svdq_mx_dequantize(p, p, 0, None, 4, 64, p, 60, 0, None) == 1
     assert L.svdq_mx_dequantize(p, p, 7, None, 4, 64, p, 64, 0, None) == 1
@@ -163,4 +171,5 @@ def test_c_abi_refusals():
         return L.svdq_rms_norm_mx(x, ldx, r, ldr, None, dt, eps, m, h, p, p, s, lds, None)
 
     assert norm(r=p) == 1 and norm(s=p) == 1 and norm(dt=4) == 1 and norm(eps=-1.0) == 1 and norm(ldx=60) == 1
+    assert norm(x=ctypes.c_void_p(4097)) == 1 and norm(r=ctypes.c_void_p(4097), s=p) == 1
     assert norm(x=None) == 1 and norm(h=0) == 1 and norm(r=p, s=p, ldr=60) == 1 and norm(m=0) == 0
