@@ -123,6 +123,7 @@ constexpr int kMaxFusedTokens = 4;
 struct MxGemm {
   int mode;
   MxInput in;
+  bool early_weight;  // the launch before this one is this call's own and does not write the weight
   int k;
   const void *a_codes, *a_scales, *w_codes, *w_scales;
   int a_fmt, w_fmt;

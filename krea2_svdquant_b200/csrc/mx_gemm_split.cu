@@ -63,6 +63,7 @@ struct SplitArgs {
   int split;    // CTAs of the cluster, a share of K each
   int stages;   // ring depth
   int n_tiles;  // tiles along the weight's rows
+  bool early_weight;
   int* err;
 };
 
@@ -200,21 +201,34 @@ __global__ void __launch_bounds__(kSplitThreads)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bars->tmem_base;
+  auto load_weight = [&](int s, int stage) {
+    const uint32_t bar = smem_u32(&bars->full[stage]), at = base + (uint32_t)(stage * S::kStage);
+    mbar_arrive_expect_tx(bar, kFused ? S::kTxFused : S::kTx);
+    tma_load_2d(at, &w_map, bar, s * 128, n0);
+    tma_load_3d(at + S::kScaleW, &sw_map, bar, 0, s * Mode::kScaleTiles, n0 / 128);
+  };
+  // Stages whose weight is on its way before the wait for the launch before this one.  That launch is the
+  // quantisation of this call's activations; it has itself waited for everything before it when
+  // this one begins, so a weight that an earlier launch wrote is in memory.
+  const int early = !kFused && a.early_weight ? min(a.stages, s1 - s0) : 0;
+  if (warp == 4 && early > 0) {
+    if (elect_one())
+      for (int i = 0; i < early; ++i) load_weight(s0 + i, i);
+    __syncwarp();
+  }
   pdl_wait();
   pdl_trigger();
 
   // producer and MMA roles: the whole warp runs the loop, one lane issues
   if (warp == 4) {
     int stage = 0;
-    uint32_t phase = 0, filled = 0, par = 0;
+    uint32_t phase = 0, filled = early > 0 ? (1u << early) - 1u : 0u, par = 0;
     bool ok = true;
     for (int s = s0; s < s1; ++s) {
       if (!(ok = warp_spin_wait(smem_u32(&bars->empty[stage]), phase ^ 1u, abort_flag, a.err, kWaitSplitEmpty))) break;
       const uint32_t bar = smem_u32(&bars->full[stage]), at = base + (uint32_t)(stage * S::kStage);
       if (elect_one()) {
-        mbar_arrive_expect_tx(bar, kFused ? S::kTxFused : S::kTx);
-        tma_load_2d(at, &w_map, bar, s * 128, n0);
-        tma_load_3d(at + S::kScaleW, &sw_map, bar, 0, s * Mode::kScaleTiles, n0 / 128);
+        if (s - s0 >= early) load_weight(s, stage);
         if (!kFused) {
           tma_load_2d(at + S::kTok, &t_map, bar, s * 128, m0);
           tma_load_3d(at + S::kScaleT, &st_map, bar, 0, s * Mode::kScaleTiles, m0 / 128);
@@ -433,6 +447,7 @@ int launch_split(const MxGemm& g, const SplitPlan& p) {
   a.err = g.err;
   a.steps = p.steps;
   a.n_tiles = p.n_tiles;
+  a.early_weight = g.early_weight;
   a.split = p.split;
   a.stages = p.stages;
   return launch_pdl("svdq_mx_gemm launch", mx_gemm_split_kernel<MODE, TN, X>, dim3((unsigned)(p.tiles * p.split)),
@@ -561,6 +576,7 @@ extern "C" int svdq_mx_linear(const void* x, int64_t ldx, int dtype, int a_forma
   uint8_t* scales = codes + mx_code_bytes(M, K, a_format);
   g.a_codes = codes;
   g.a_scales = scales;
+  g.early_weight = true;
   const int st = svdq_mx_quantize(x, ldx, dtype, M, K, a_format, a_tensor_scale, codes, scales, stream);
   return st ? st : mx_product(g, K);
 }

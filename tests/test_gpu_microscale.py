@@ -429,6 +429,28 @@ def test_few_tokens_quantised_by_the_product(act, w_fmt, dtype, m, n, k, cut):
     no_device_error()
 
 
+@pytest.mark.parametrize("act,w_fmt", PRODUCTS)
+@pytest.mark.parametrize("m", [4, 16, 64, 300])
+def test_weight_written_just_before_the_call(act, w_fmt, m):
+    """A weight that the launch before the linear writes (a quantisation, a copy) is the one it reads."""
+    M = ms()
+    x = data(m, 2048, torch.bfloat16)
+    sources = [data(2000, 2048, torch.bfloat16, seed=i, scale=0.1) for i in range(3)]
+    weights = [M.quantize(s, w_fmt) for s in sources]
+    want = [M.matmul(M.quantize(x, act), w) for w in weights]
+    torch.cuda.synchronize()
+    w = M.MicroTensor(weights[0].codes.clone(), weights[0].scales.clone(), w_fmt, weights[0].shape)
+    got, fresh = [], []
+    for i in range(30):
+        w.codes.copy_(weights[i % 3].codes)
+        w.scales.copy_(weights[i % 3].scales)
+        got.append(M.linear(x, w, act=act))
+        fresh.append(M.linear(x, M.quantize(sources[i % 3], w_fmt), act=act))
+    for i in range(30):
+        assert torch.equal(got[i], want[i % 3]) and torch.equal(fresh[i], want[i % 3])
+    no_device_error()
+
+
 def test_registered_ops():
     """The operators as torch custom ops: the same results, shapes under fake tensors, and a compiled call."""
     from krea2_svdquant_b200 import ops
