@@ -111,10 +111,9 @@ __device__ __forceinline__ uint32_t e2m1_of(double q) {
   const uint32_t c = (a > 0.25) + (a >= 0.75) + (a > 1.25) + (a >= 1.75) + (a > 2.5) + (a >= 3.5) + (a > 5.0);
   return c | (signbit(q) ? 8u : 0u);
 }
-// An nvfp4 block whose scale or values are near the ends of fp32's range, in 64 bits.  Takes -x.  Rare:
-// one element at a time, picked out of registers, so that it costs the usual path neither
-// registers nor a stack.
-__device__ __forceinline__ uint2 nvfp4_codes_wide(const float (&nx)[16], float sf, float g) {
+// An nvfp4 block whose scale or values are near the ends of fp32's range, in 64 bits.  Rare: one element
+// at a time, picked out of registers, so that it costs the usual path neither registers nor a stack.
+__device__ __forceinline__ uint2 nvfp4_codes_wide(const float (&x)[16], float sf, float g) {
   const double d = (double)sf * (double)g;
   uint2 w = make_uint2(0u, 0u);
 #pragma unroll 1
@@ -122,7 +121,7 @@ __device__ __forceinline__ uint2 nvfp4_codes_wide(const float (&nx)[16], float s
     float v = 0.0f;
 #pragma unroll
     for (int j = 0; j < 16; ++j)
-      if (j == i) v = -nx[j];
+      if (j == i) v = x[j];
     const uint32_t c = e2m1_of((double)v / d) << (4 * (i & 7));
     if (i < 8) w.x |= c;
     else w.y |= c;
@@ -132,76 +131,96 @@ __device__ __forceinline__ uint2 nvfp4_codes_wide(const float (&nx)[16], float s
 
 // What the quotients of an nvfp4 block need, by its scale byte.  A launch has one tensor scale g, so a
 // CTA works this out once per byte.
+enum : uint32_t { kTimesY = 0, kQuotient = 1, kQuotientOdd = 2 };
 struct Nvfp4Unit {
-  float d;        // the divisor: sf g, or a neighbour of it (below)
-  float ny;       // -1 / d, rounded
-  float limit;    // magnitudes up to this take the fp32 quotient (below 0: none)
-  uint32_t odd;   // quotients on a border have to be checked
+  float d;        // fl32(sf g)
+  float y;        // kTimesY: the factor that stands for 1 / (sf g); otherwise 1 / d, rounded
+  float limit;    // magnitudes up to this take fp32 (below 0: none)
+  uint32_t how;
 };
 
-// Codes are e2m1(x / (sf g)) of the exact quotient.  The correctly rounded x / fl32(sf g) decides them
-// unless it lands on a border b between two codes that the exact quotient only comes close to.  For x
-// of P significant bits (8 in bf16, 11 in fp16) that takes an x within 2^-22 of b sf g; b's
-// significand is m / 4 with m = 4 .. 7, so one x per m and power of two: x_m, m sf g rounded to P
-// bits.  All x_m 2^k lie on the same side of their borders, so a divisor moved by 2^-20 to that side
-// decides them, and no other x is near enough to a border for that to matter if every other m sf g is
-// 2^-18 from its x_m.  Where that does not hold, and for fp32 (P = 24), quotients that have at most 3
-// significant bits, as borders do, are moved to odd one by one.
-// (Common, not an accident: g = amax / 2688 = amax / (7 * 384) with a short amax brings every 7 sf g
-// next to a short number.)
+// Codes are e2m1(x / (sf g)) of the exact quotient, ties to even.  For x of P significant bits (8 in
+// bf16, 11 in fp16) few x matter: a border b between two codes has the significand m / 4, m = 4 .. 7,
+// and only x_m 2^k, x_m = m sf g rounded to P bits, can come close to b sf g.  All x_m 2^k of one m lie on
+// the same side of their borders, and where they lie on them, ties to even go down for m = 4 and 5
+// and up for 6 and 7.  So where the x_m that come within 2^-20 of their borders all want one side, and the
+// others keep 2^-17 away, x times the reciprocal of sf g moved by 2^-19 to that side decides every
+// code (its rounding errors are below 2^-22).  Otherwise the correctly rounded quotient x / d does,
+// unless d is not sf g or an x_m is close to its border without being on it; then, and for fp32 (P = 24),
+// quotients that have at most 3 significant bits, as borders do, are moved to odd one by one.
+// (Sides matter often: g = amax / 2688 = amax / (7 * 384) with a short amax brings every 7 sf g next to
+// a short number, and g = 1 puts every x_m on its border.  4352 x 6144 bf16: 16.5 us with one product,
+// 18.0 with the quotient.)
 template <int P>
 __device__ __forceinline__ Nvfp4Unit nvfp4_unit(uint32_t byte, float g) {
   const float sf = e4m3_value(byte);
   const float d = sf * g, dl = fmaf(sf, g, -d);
-  Nvfp4Unit u{d, 0.0f, -1.0f, 0u};
+  Nvfp4Unit u{d, 0.0f, -1.0f, kQuotientOdd};
   if (!(d >= 8.0e-28f && d <= 1.0e30f)) return u;  // 64 bits
   u.limit = d * 65536.0f;
+  u.y = __frcp_rn(d);
   if constexpr (P < 24) {
-    bool up = false, down = false, between = false;
+    bool up = false, down = false, between = false, beside = dl != 0.0f;
 #pragma unroll
     for (int m = 4; m <= 7; ++m) {
       constexpr uint32_t drop = 24 - P;
       const float xm = __uint_as_float((__float_as_uint((float)m * d) + (1u << (drop - 1))) & ~((1u << drop) - 1u));
       const float delta = fmaf((float)m, d, -xm) + (float)m * dl;
-      const bool close = fabsf(delta) < xm * 0x1p-22f && delta != 0.0f;
-      up |= close && delta > 0.0f;
-      down |= close && delta < 0.0f;
-      between |= !close && fabsf(delta) < xm * 0x1p-18f;
+      const float off = fabsf(delta);
+      if (off < xm * 0x1p-20f) {
+        const bool to_down = delta != 0.0f ? delta > 0.0f : m < 6;
+        up |= !to_down;
+        down |= to_down;
+        beside |= delta != 0.0f;
+      } else {
+        between |= off < xm * 0x1p-17f;
+      }
     }
-    if ((up && down) || ((up || down) && between)) u.odd = 1u;
-    else if (up) u.d = d * (1.0f + 0x1p-20f);
-    else if (down) u.d = d * (1.0f - 0x1p-20f);
-  } else {
-    u.odd = 1u;
+    if (!(up && down) && !((up || down) && between)) {
+      u.how = kTimesY;
+      if (up) u.y *= 1.0f + 0x1p-19f;
+      if (down) u.y *= 1.0f - 0x1p-19f;
+    } else if (!beside) {
+      u.how = kQuotient;
+    }
   }
-  u.ny = -__frcp_rn(u.d);
   return u;
 }
 
-// 16 values of an nvfp4 block as codes.  Takes -x: with q0 = (-x)(-y), r = q0 d - x and q = q0 - r y a
-// zero keeps its sign.
-__device__ __forceinline__ uint2 nvfp4_codes(const float (&nx)[16], uint32_t amax_bits, uint32_t byte,
+// 16 values of an nvfp4 block as codes.
+__device__ __forceinline__ uint2 nvfp4_codes(const float (&x)[16], uint32_t amax_bits, uint32_t byte,
                                              const Nvfp4Unit& u, float g) {
   if (byte == 0u || byte == 0x7Fu) return make_uint2(0u, 0u);
-  if (!(__uint_as_float(amax_bits) <= u.limit)) return nvfp4_codes_wide(nx, e4m3_value(byte), g);
-  const uint64_t ny = f2_pack(u.ny, u.ny), dd = f2_pack(u.d, u.d);
+  if (!(__uint_as_float(amax_bits) <= u.limit)) return nvfp4_codes_wide(x, e4m3_value(byte), g);
   float q[16];
+  if (u.how == kTimesY) {
+    const uint64_t yy = f2_pack(u.y, u.y);
 #pragma unroll
-  for (int i = 0; i < 16; i += 2) {
-    const uint64_t xx = f2_pack(nx[i], nx[i + 1]);
-    const uint64_t q0 = f2_mul(xx, ny);
-    const uint64_t qq = f2_fma(f2_fma(q0, dd, xx), ny, q0);
-    q[i] = f2_lo(qq);
-    q[i + 1] = f2_hi(qq);
-  }
-  if (u.odd) {
-    bool near_border = false;
+    for (int i = 0; i < 16; i += 2) {
+      const uint64_t p = f2_mul(f2_pack(x[i], x[i + 1]), yy);
+      q[i] = f2_lo(p);
+      q[i + 1] = f2_hi(p);
+    }
+  } else {
+    // Markstein's correction with -x: q0 = (-x)(-y), r = q0 d - x, q = q0 - r y, so that a zero keeps its sign
+    const uint64_t ny = f2_pack(-u.y, -u.y), dd = f2_pack(u.d, u.d);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) near_border |= (__float_as_uint(q[i]) & 0x1FFFFFu) == 0u;
-    if (near_border) {
-      const float dl = fmaf(e4m3_value(byte), g, -u.d);
+    for (int i = 0; i < 16; i += 2) {
+      const uint64_t xx = f2_pack(-x[i], -x[i + 1]);
+      const uint64_t q0 = f2_mul(xx, ny);
+      const uint64_t p = f2_fma(f2_fma(q0, dd, xx), ny, q0);
+      q[i] = f2_lo(p);
+      q[i + 1] = f2_hi(p);
+    }
+    if (u.how == kQuotientOdd) {
+      bool near_border = false;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) q[i] = to_odd(q[i], -nx[i], u.d, dl);
+      for (int i = 0; i < 16; ++i) near_border |= (__float_as_uint(q[i]) & 0x1FFFFFu) == 0u;
+      if (near_border) {
+        const float dl = fmaf(e4m3_value(byte), g, -u.d);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) q[i] = to_odd(q[i], x[i], u.d, dl);
+      }
     }
   }
   return make_uint2(e2m1x8_satfinite(q), e2m1x8_satfinite(q + 8));
@@ -394,16 +413,13 @@ __device__ __forceinline__ typename CodeWord<FMT>::type mx_codes(const T (&x)[16
     return make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
-// The codes of 16 columns (x is overwritten) and their block's scale byte.  An mx block is shared with
+// The codes of 16 columns and their block's scale byte.  An mx block is shared with
 // the neighbouring lane (lane ^ 1), so every lane of the warp takes part.
 template <typename T, int FMT>
-__device__ __forceinline__ typename CodeWord<FMT>::type encode_chunk(T (&x)[16], float g, const Nvfp4Unit* units,
+__device__ __forceinline__ typename CodeWord<FMT>::type encode_chunk(const T (&x)[16], float g, const Nvfp4Unit* units,
                                                                      uint32_t& byte) {
   uint32_t amax = amax_bits_of(x);
-  if constexpr (FMT == kNvfp4) {  // nvfp4_codes takes -x
-    constexpr uint32_t kSigns = sizeof(T) == 2 ? 0x80008000u : 0x80000000u;
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(T) * 4; ++i) reinterpret_cast<uint32_t*>(x)[i] ^= kSigns;
+  if constexpr (FMT == kNvfp4) {
     float v[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) v[i] = to_float(x[i]);

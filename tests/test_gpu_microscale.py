@@ -137,6 +137,26 @@ def test_borders_with_a_tensor_scale_of_24_bits():
     check_quantized(ms().quantize(xt, "nvfp4", tensor_scale=torch.tensor([g], device="cuda")), xt, "nvfp4", float(g))
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("g", [1.0, 0.75, 90 / 2688, 15 / 448, 13.25 / 2688, 1 / 3, 0.1, 0.0371, 1 + 2.0 ** -23, 1 + 2.0 ** -9,
+                               0.25 * (1 + 2.0 ** -17), 0.25 * (1 - 2.0 ** -19), 8 / 7, 1 / 7 + 2.0 ** -26, 4 / 5 - 2.0 ** -22])
+def test_borders_of_16_bit_inputs(dtype, g):
+    """The 16-bit numbers nearest to every border times every scale times g, and their neighbours: tensor scales
+    that put none, one, some or all of them on their borders, exactly or nearly."""
+    t, g = DTYPES[dtype], np.float32(g)
+    sf = O.E4M3[16:120]
+    mid = (O.E2M1[1:8] + O.E2M1[:7]) / 2
+    unit = (sf * np.float64(g))[:, None]
+    x = torch.from_numpy(unit * mid).to(t)
+    near = x.view(torch.int16)
+    rows = torch.cat([x, (near + 1).view(t), (near - 1).view(t)], 1)  # 21 a scale, in two blocks of 16
+    rows = torch.cat([rows[:, :11], rows[:, 11:], -rows[:, :8]], 1)[:, :30]
+    top = torch.from_numpy(unit * 6).to(t)
+    blocks = torch.cat([top, rows[:, :15], top, rows[:, 15:]], 1).contiguous()
+    check_quantized(ms().quantize(blocks.cuda(), "nvfp4", tensor_scale=torch.tensor([g], device="cuda")), blocks,
+                    "nvfp4", float(g))
+
+
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
 def test_extreme_values(fmt, dtype):
