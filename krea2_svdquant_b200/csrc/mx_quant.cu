@@ -41,17 +41,17 @@ struct QuantArgs {
   uint8_t* scales;
 };
 
-// A thread quantises 64 bytes of a row: 32 columns of a 16-bit type, which are two nvfp4 blocks or one mx
-// block, or 16 columns in fp32, one nvfp4 block or half an mx block whose other half is the
-// neighbouring lane's.  HBM moves 2 bytes in and 0.5 out per element from bf16 to a 4-bit
-// format; the instructions for them are nearly as much work, so what is done once per thread is shared
-// by as many columns as stay in registers (16 columns a thread: 13.0 us to mxfp4, 32: 11.6, which is 5.8
-// TB/s; to nvfp4 the instructions bound it, 17 us or 4.0 TB/s, all at 4352 x 6144 from bf16).  The four scale bytes of a 32-bit word of the tile
-// layout come from 2 to 8 neighbouring lanes and leave as one store.
+// A thread quantises 64 bytes of a row: 32 columns of a 16-bit type, which are two nvfp4 blocks or one
+// mx block, or 16 columns in fp32, one nvfp4 block or half an mx block whose other half is the
+// neighbouring lane's.  HBM moves 2 bytes in and 0.5 out per element from bf16 to a 4-bit format;
+// the instructions for them are nearly as much work, so what is done once per thread is shared by as
+// many columns as stay in registers.  4352 x 6144 from bf16: to mxfp4 13.0 us with 16 columns a thread,
+// 11.6 us (5.8 TB/s) with 32; to nvfp4 17 us (4.0 TB/s), bound by the instructions.  The four scale
+// bytes of a 32-bit word of the tile layout come from 2 to 8 neighbouring lanes and leave as one store.
 //
 // A CTA takes kThreads neighbouring chunks.  From fp32 to nvfp4 it stays for a share of the launch's
 // chunks, with the loads of the next ones issued before the present ones are worked on, because its
-// units cost as much as half a step (4352 x 6144: 21.8 us against 25.5); the others run faster one
+// units cost as much as half a step (4352 x 6144: 21.6 us against 25.5); the others run faster one
 // step to a CTA (from bf16 to nvfp4 18.1 us against 20.4 when that was tried).  VEC: rows on 32-byte
 // boundaries and K a multiple of 16.
 template <typename T, int FMT>
