@@ -471,6 +471,26 @@ def test_weight_written_just_before_the_call(act, w_fmt, m):
     no_device_error()
 
 
+@pytest.mark.parametrize("m", [4, 16, 300])
+def test_captured_with_the_weight_written_before(m):
+    """A captured copy of the weight, or its quantisation, and the linear behind it, replayed with other weights."""
+    M = ms()
+    x, src = data(m, 1024, torch.bfloat16), data(1000, 1024, torch.bfloat16, seed=5, scale=0.1)
+    w = M.quantize(src, "nvfp4")
+    codes, graph = w.codes.clone(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        w.codes.copy_(codes)
+        copied = M.linear(x, w)
+        fresh = M.linear(x, M.quantize(src, "nvfp4"))
+    for i in range(10):
+        codes.copy_(torch.roll(codes, 1, 0))
+        src.copy_(torch.roll(src, 1, 1))
+        graph.replay()
+        assert torch.equal(copied, M.matmul(M.quantize(x, "nvfp4"), M.MicroTensor(codes, w.scales, "nvfp4", w.shape)))
+        assert torch.equal(fresh, M.matmul(M.quantize(x, "nvfp4"), M.quantize(src, "nvfp4")))
+    no_device_error()
+
+
 def test_registered_ops():
     """The operators as torch custom ops: the same results, shapes under fake tensors, and a compiled call."""
     from krea2_svdquant_b200 import ops
