@@ -112,7 +112,9 @@ __device__ __forceinline__ void store32(void* p, const uint32_t (&w)[8]) {
 }
 
 // 32 x 32 outputs from the accumulator: lane l holds row m0 + l, columns n .. n + 31.  Where the
-// rows allow it each lane writes its row in 32-byte pieces; otherwise (N or the output's address
+// rows allow it each lane writes its row in 32-byte pieces (through shared memory and TMA stores
+// instead, M 4352, N 16384, nvfp4: 50 us against 49 at K 1024, 194 against 160 at K 6144; a short K is
+// bound by writing the output); otherwise (N or the output's address
 // is not a multiple of 32 bytes, or columns are missing) the chunk is turned in shared memory and
 // each row leaves as 32 neighbouring elements.
 __device__ __forceinline__ void store_chunk(const MxOutput& o, int m0, int lane, int n, const uint32_t (&acc)[32],
@@ -316,7 +318,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       const int m0 = mb * 2 * BM + (int)rank * BM + (warp & 3) * 32, n0 = nb * BN;
       const int first = (j & 1) ? half : 6 + half;  // the chunk in the columns that the accumulators share
       const uint32_t acc = lanes + (uint32_t)((j & 1) * kAccShift);
-      if (!mbar_spin_wait(smem_u32(&bars->acc_full[j & 1]), (uint32_t)(j >> 1) & 1u, abort_flag, a.err, kWaitPairEpi))
+      if (!warp_spin_wait(smem_u32(&bars->acc_full[j & 1]), (uint32_t)(j >> 1) & 1u, abort_flag, a.err, kWaitPairEpi))
         break;
       tc_fence_after();
       uint32_t va[32], vb[32];

@@ -290,7 +290,8 @@ __global__ void __launch_bounds__(kSplitThreads)
   const int row = warp * 32 + lane, n = n0 + row;
   bool ok = true;
   if (warp < 4) {
-    ok = mbar_spin_wait(smem_u32(&bars->done), 0, abort_flag, a.err, kWaitSplitEpi) && !*abort_flag;
+    ok = warp_spin_wait(smem_u32(&bars->done), 0, abort_flag, a.err, kWaitSplitEpi);
+    ok = __all_sync(0xffffffffu, ok && !*abort_flag);
     tc_fence_after();
   }
   const float alpha = mx_alpha(a.o);
