@@ -173,3 +173,53 @@ def test_c_abi_refusals():
     assert norm(r=p) == 1 and norm(s=p) == 1 and norm(dt=4) == 1 and norm(eps=-1.0) == 1 and norm(ldx=60) == 1
     assert norm(x=ctypes.c_void_p(4097)) == 1 and norm(r=ctypes.c_void_p(4097), s=p) == 1
     assert norm(x=None) == 1 and norm(h=0) == 1 and norm(r=p, s=p, ldr=60) == 1 and norm(m=0) == 0
+
+
+def test_a_launch_makes_its_device_current(monkeypatch):
+    """A launch for another device than the current one runs inside that device's guard, on its stream."""
+    seen, here = [], [0]
+
+    class Lib:
+        def svdq_probe(self, *args):
+            seen.append((here[0], args))
+            return 0
+
+    class Guard:
+        def __init__(self, dev):
+            self.dev = dev
+
+        def __enter__(self):
+            self.was, here[0] = here[0], self.dev.index
+
+        def __exit__(self, *exc):
+            here[0] = self.was
+
+    monkeypatch.setattr(ops._lib, "lib", lambda: Lib())
+    monkeypatch.setattr(ops, "_current_device", lambda: here[0])
+    monkeypatch.setattr(ops, "_current_stream", lambda i: 100 + i)
+    monkeypatch.setattr(ops, "_raw_stream", lambda dev: 100 + dev.index)
+    monkeypatch.setattr(torch.cuda, "device", Guard)
+    ops._launch(torch.device("cuda", 0), "svdq_probe", 7)
+    ops._launch(torch.device("cuda", 1), "svdq_probe", 8)
+    assert seen == [(0, (7, 100)), (1, (8, 101))] and here[0] == 0
+
+
+def test_a_failing_launch_raises_the_library_error(monkeypatch):
+    monkeypatch.setattr(ops, "_current_device", lambda: 0)
+    monkeypatch.setattr(ops, "_current_stream", lambda i: None)
+    with pytest.raises(_lib.SVDQError, match="format"):
+        ops._launch(torch.device("cuda", 0), "svdq_mx_quantize", 4096, 64, 0, 4, 64, 9, None, 4096, 4096)
+
+
+def test_rows_of_any_layout_are_taken_or_copied():
+    x = torch.arange(60.0).view(5, 12)
+    assert M._rows(x) is x and M._rows(x[:, 2:9]).data_ptr() == x[:, 2:9].data_ptr()
+    for v in (x.t(), x[:1].expand(4, 12), x[:, ::2], x[None, :, 3:], x[0], x[:, 4]):
+        r = M._rows(v)
+        assert r.dim() == 2 and torch.equal(r.reshape(v.shape), v)
+        ops._mx_rows("t", r)
+    with pytest.raises(ValueError, match="dimension"):
+        M._rows(torch.tensor(1.0))
+    for bad in (x.double(), x.int(), x[0], x.t(), x[:1].expand(4, 12), x[:, :0]):
+        with pytest.raises(ValueError):
+            ops._mx_rows("t", bad)
