@@ -2,10 +2,11 @@
 // scale per 32 columns):
 //   h = x + residual, rounded to its type and stored;   y = h * rsqrt(mean(h^2) + eps) * weight
 //   scale = 2^(floor(log2 max|y|) - 8) per 32 columns,  code = e4m3(y / scale)
-// The norm reads h as it is stored, so a residual stream read back later gives the same norm.  Squares
-// are summed in fp32 within a thread and in 64 bits over the row, the root is held as the sum of two
-// fp32 values, and h * weight is exact in fp32 for 16-bit types: y is rounded to fp32 once before it
-// is rounded to its code, so that hardly a code or a scale falls on the other side of a border.
+// The norm reads h as it is stored, so a residual stream read back later gives the same norm.
+//
+// y is worked out in fp32 where that holds the squares, their root and h * weight.  Rows far from one, and
+// blocks of which it does not hold the product, are done in 64 bits, up to the ends of the type's range
+// (a y past fp32's own is an infinity).
 #include "mx_common.cuh"
 
 namespace svdq {
@@ -25,6 +26,66 @@ struct NormArgs {
   void* sum;
   int64_t lds;
 };
+
+// C = 32 bytes of a row's columns; zero from column H on.
+template <bool VEC, typename T, int C>
+__device__ __forceinline__ void load_columns(const T* row, int c, int H, T (&v)[C]) {
+  if constexpr (!VEC) {
+    load_shifted(row, c, H, v);
+  } else if (c < H) {
+    load_vec(row + c, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < C; ++i) v[i] = from_float<T>(0.0f);
+  }
+}
+// Bits of the largest magnitude of an mx block, from the 32 / C neighbouring lanes that have it.
+template <int C>
+__device__ __forceinline__ uint32_t block_max(const float (&y)[C]) {
+  uint32_t amax = amax_bits_of(y);
+  amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+  if (C == 8) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+  return amax;
+}
+template <int W>
+__device__ __forceinline__ void store_codes(const NormArgs& a, int row, int c, const uint32_t (&q)[W], uint32_t byte) {
+  constexpr int L = 8 / W;  // lanes per block
+  const int lane = threadIdx.x & 31, words = a.h_pad / 128;
+  uint32_t word = byte << (8 * ((lane / L) & 3));
+  word |= __shfl_xor_sync(0xffffffffu, word, L);
+  word |= __shfl_xor_sync(0xffffffffu, word, 2 * L);
+  if (c < a.h_pad) {
+    uint8_t* to = a.codes + (size_t)row * a.h_pad + c;
+    if constexpr (W == 4) *reinterpret_cast<uint4*>(to) = make_uint4(q[0], q[1], q[2], q[3]);
+    else *reinterpret_cast<uint2*>(to) = make_uint2(q[0], q[1]);
+    if (lane % (4 * L) == 0) *reinterpret_cast<uint32_t*>(a.scales + mx_scale_word(row, c >> 7, words)) = word;
+  }
+}
+
+// The codes of a warp's columns (c is the lane's) in 64 bits, from the row as it is stored.
+template <typename T, bool VEC>
+__device__ __forceinline__ void encode_exactly(const NormArgs& a, int row, const T* h_row, int c, double root) {
+  constexpr int C = 32 / (int)sizeof(T);
+  alignas(32) T h[C], w[C];
+  load_columns<VEC>(h_row, c, a.H, h);
+  if (a.weight) load_columns<VEC>(static_cast<const T*>(a.weight), c, a.H, w);
+  float y[C];
+#pragma unroll
+  for (int i = 0; i < C; ++i) {
+    double d = (double)to_float(h[i]);
+    if (a.weight) d *= (double)to_float(w[i]);
+    y[i] = (float)(d * root);
+  }
+  const uint32_t byte = mx_scale_byte<kMxfp8>(block_max(y));
+  if (byte == 255u) {
+#pragma unroll
+    for (int i = 0; i < C; ++i) y[i] = 0.0f;
+  }
+  scale_all(y, mx_inverse_scale(byte));
+  uint32_t q[C / 4];
+  e4m3_words(y, q);
+  store_codes(a, row, c, q, byte);
+}
 
 // One CTA per row.  A thread owns C columns of each C * THREADS (C = 16, or 8 in fp32: 32 bytes); the
 // 32 / C neighbouring lanes of an mx block share its scale.  The row stays in registers between the
@@ -52,31 +113,32 @@ __global__ void __launch_bounds__(THREADS) rms_norm_mx_kernel(const NormArgs a) 
   const T* weight = static_cast<const T*>(a.weight);
   const int passes = PASSES > 0 ? PASSES : (a.h_pad + C * THREADS - 1) / (C * THREADS);
   auto column = [&](int p) { return (p * THREADS + tid) * C; };
-  auto load = [&](const T* p, int c, T (&v)[C]) {
-    if constexpr (!VEC) {
-      load_shifted(p, c, a.H, v);
-    } else if (c < a.H) {
-      load_vec(p + c, v);
-    } else {
-#pragma unroll
-      for (int i = 0; i < C; ++i) v[i] = from_float<T>(0.0f);
-    }
-  };
+  auto load = [&](const T* p, int c, T (&v)[C]) { load_columns<VEC>(p, c, a.H, v); };
   alignas(32) T keep[kKeep][C];
   alignas(32) T res[kKeep][C];
-  uint64_t ss2 = 0;  // two sums of squares
-  auto add = [&](int c, T (&h)[C], const T (&r)[C]) {
+  double ss = 0.0;
+  auto pass_bit = [](int p) { return 1u << (PASSES > 0 || p < 31 ? p : 31); };  // the last one is of all the rest
+  uint32_t some = 0;  // passes of which this thread has an element that is not zero
+  auto add = [&](int p, T (&h)[C], const T (&r)[C]) {
+    const int c = column(p);
     if (rr) {
 #pragma unroll
       for (int i = 0; i < C; ++i) h[i] = from_float<T>(to_float(h[i]) + to_float(r[i]));
       if constexpr (!VEC) store_warp(sr, c, a.H, stage + (tid & ~31) * C, h);
       else if (c < a.H) store_vec(sr + c, h);
     }
+    uint64_t s2[2] = {0, 0};  // C / 4 squares each, and 64 bits from there on: off by (C / 4 + 1) 2^-24 at most
 #pragma unroll
     for (int i = 0; i < C; i += 2) {
       const uint64_t v = f2_pack(to_float(h[i]), to_float(h[i + 1]));
-      ss2 = f2_fma(v, v, ss2);
+      s2[i / 2 % 2] = f2_fma(v, v, s2[i / 2 % 2]);
     }
+    const uint64_t both = f2_add(s2[0], s2[1]);
+    ss += (double)f2_lo(both) + (double)f2_hi(both);
+    uint32_t bits = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) bits |= reinterpret_cast<const uint32_t*>(h)[i];
+    some |= (bits & (sizeof(T) == 2 ? 0x7FFF7FFFu : 0x7FFFFFFFu)) != 0u ? pass_bit(p) : 0u;
   };
   if constexpr (PASSES > 0) {  // every load first
 #pragma unroll
@@ -86,71 +148,81 @@ __global__ void __launch_bounds__(THREADS) rms_norm_mx_kernel(const NormArgs a) 
       for (int p = 0; p < PASSES; ++p) load(rr, column(p), res[p]);
     }
 #pragma unroll
-    for (int p = 0; p < PASSES; ++p) add(column(p), keep[p], res[p]);
+    for (int p = 0; p < PASSES; ++p) add(p, keep[p], res[p]);
   } else {
     for (int p = 0; p < passes; ++p) {
       load(xr, column(p), keep[0]);
       if (rr) load(rr, column(p), res[0]);
-      add(column(p), keep[0], res[0]);
+      add(p, keep[0], res[0]);
     }
   }
-  double ss = (double)f2_lo(ss2) + (double)f2_hi(ss2);
+  auto over_row = [&](double t) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  if (lane == 0) part[tid >> 5] = ss;
-  __syncthreads();
-  ss = 0.0;
+    for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+    if (lane == 0) part[tid >> 5] = t;
+    __syncthreads();
+    t = 0.0;
 #pragma unroll
-  for (int w = 0; w < THREADS / 32; ++w) ss += part[w];
-  // 1 / sqrt(v) as hi + lo: hi = fp32 of it to a few ulp, lo = hi (1 - v hi^2) / 2 (a Newton step)
-  const double v = fma(ss, a.per_column, (double)a.eps);
-  const float hi = 1.0f / sqrtf((float)v);
-  const float lo = 0.5f * hi * (float)fma(-v, (double)hi * (double)hi, 1.0);
-  const uint64_t hi2 = f2_pack(hi, hi), lo2 = isfinite(hi) && hi != 0.0f ? f2_pack(lo, lo) : 0;
-  auto encode = [&](int c, const T (&h)[C]) {
+    for (int w = 0; w < THREADS / 32; ++w) t += part[w];
+    return t;
+  };
+  // Between 2^-60 and 2^60 no square was infinite, and what those below fp32's normal range lost does not count.
+  const double v = fma(over_row(ss), a.per_column, (double)a.eps);
+  const bool near_one = v >= 0x1p-60 && v <= 0x1p60;
+  const float root = near_one ? 1.0f / sqrtf((float)v) : 1.0f;
+  const uint64_t root2 = f2_pack(root, root);
+
+  // In fp32.  The pass's bit where that does not hold a value.
+  auto encode = [&](int p, const T (&h)[C]) {
+    const int c = column(p);
     alignas(32) T w[C];
     if (weight) load(weight, c, w);
     float y[C];
 #pragma unroll
     for (int i = 0; i < C; i += 2) {
-      uint64_t p = f2_pack(to_float(h[i]), to_float(h[i + 1]));
-      if (weight) p = f2_mul(p, f2_pack(to_float(w[i]), to_float(w[i + 1])));
-      p = f2_fma(p, hi2, f2_mul(p, lo2));
-      y[i] = f2_lo(p);
-      y[i + 1] = f2_hi(p);
+      uint64_t v2 = f2_pack(to_float(h[i]), to_float(h[i + 1]));
+      if (weight) v2 = f2_mul(v2, f2_pack(to_float(w[i]), to_float(w[i + 1])));
+      v2 = f2_mul(v2, root2);
+      y[i] = f2_lo(v2);
+      y[i + 1] = f2_hi(v2);
     }
-    uint32_t amax = amax_bits_of(y);
-    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-    if (C == 8) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+    const uint32_t amax = block_max(y);
+    // From 2^-60 on a block's codes do not see what an h * weight below fp32's normal range lost (2^-150; in y
+    // 2^-120); an infinite one, or a NaN, shows in amax.
+    const bool unsure = !near_one || amax >= 0x7F800000u || (amax < 0x21800000u && (some & pass_bit(p)) != 0u);
     const uint32_t byte = mx_scale_byte<kMxfp8>(amax);
-    if (byte == 255u) {
-#pragma unroll
-      for (int i = 0; i < C; ++i) y[i] = 0.0f;
-    }
     scale_all(y, mx_inverse_scale(byte));
     uint32_t q[C / 4];
     e4m3_words(y, q);
-    constexpr int L = 32 / C;  // lanes per block
-    uint32_t word = byte << (8 * ((lane / L) & 3));
-    word |= __shfl_xor_sync(0xffffffffu, word, L);
-    word |= __shfl_xor_sync(0xffffffffu, word, 2 * L);
-    if (c < a.h_pad) {
-      uint8_t* to = a.codes + (size_t)row * a.h_pad + c;
-      if constexpr (C == 16) *reinterpret_cast<uint4*>(to) = make_uint4(q[0], q[1], q[2], q[3]);
-      else *reinterpret_cast<uint2*>(to) = make_uint2(q[0], q[1]);
-      if (lane % (4 * L) == 0) *reinterpret_cast<uint32_t*>(a.scales + mx_scale_word(row, c >> 7, words)) = word;
-    }
+    store_codes(a, row, c, q, byte);
+    return unsure ? pass_bit(p) : 0u;
   };
+  const T* h_row = sr ? sr : xr;  // the sums as this warp stored them
+  uint32_t again = 0;             // passes that the warp works out again
   if constexpr (PASSES > 0) {
 #pragma unroll
-    for (int p = 0; p < PASSES; ++p) encode(column(p), keep[p]);
+    for (int p = 0; p < PASSES; ++p) again |= encode(p, keep[p]);
   } else {
     for (int p = 0; p < passes; ++p) {
       if constexpr (!VEC) __syncwarp();
-      load(sr ? sr : xr, column(p), keep[0]);  // the sums as this warp stored them
-      encode(column(p), keep[0]);
+      load(h_row, column(p), keep[0]);
+      again |= encode(p, keep[0]);
     }
   }
+  again = __reduce_or_sync(0xffffffffu, again);
+  if (!__syncthreads_or((int)again)) return;
+  double t[4] = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll 1
+  for (int p = 0; p < passes; ++p) {
+    alignas(32) T h[C];
+    load(h_row, column(p), h);
+#pragma unroll
+    for (int i = 0; i < C; ++i) t[i & 3] = fma((double)to_float(h[i]), (double)to_float(h[i]), t[i & 3]);
+  }
+  const double exact = 1.0 / sqrt(fma(over_row((t[0] + t[1]) + (t[2] + t[3])), a.per_column, (double)a.eps));
+#pragma unroll 1
+  for (int p = 0; p < passes; ++p)
+    if (again & pass_bit(p)) encode_exactly<T, VEC>(a, row, h_row, column(p), exact);
 }
 
 template <typename T, bool VEC>
