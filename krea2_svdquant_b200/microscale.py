@@ -115,8 +115,8 @@ def linear(x: torch.Tensor | MicroTensor, w: MicroTensor, bias: torch.Tensor | N
 def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, *, residual: torch.Tensor | None = None,
              eps: float = 1e-6) -> tuple[MicroTensor, torch.Tensor]:
     """``(norm, h)``: ``h = x + residual`` in x's dtype (x itself without a residual) and the
-    root-mean-square norm ``h * rsqrt(mean(h^2) + eps) * weight`` over the last dimension, kept in
-    fp32 until it is rounded to mxfp8."""
+    root-mean-square norm ``h * rsqrt(mean(h^2) + eps) * weight`` over the last dimension as mxfp8, with
+    the codes and scales of its exact value."""
     x2 = _rows(x)
     if residual is not None and residual.shape != x.shape:
         raise ValueError(f"rms_norm: residual {tuple(residual.shape)} must have x's shape {tuple(x.shape)}")
