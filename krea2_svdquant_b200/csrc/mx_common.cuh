@@ -72,8 +72,8 @@ __device__ __forceinline__ float mx_inverse_scale(uint32_t byte) {
   return byte == 255 ? 0.0f : __uint_as_float((254u - byte) << 23);
 }
 
-// The correctly rounded quotient q = x / h, moved to odd: where x / (h + l) is not exactly q, the
-// neighbour of q on its side, or q itself, whose last bit is set.  Rounding that to a type with at
+// A quotient q within a hair more than half a step of x / (h + l), moved to odd: where x / (h + l) is not exactly
+// q, the neighbour of q on its side, or q itself, whose last bit is set.  Rounding that to a type with at
 // least two bits fewer gives the rounding of the exact quotient.
 __device__ __forceinline__ float to_odd(float q, float x, float h, float l) {
   const float r = fmaf(-q, l, fmaf(-q, h, x));  // x - q (h + l): the inner difference is exact
@@ -81,11 +81,12 @@ __device__ __forceinline__ float to_odd(float q, float x, float h, float l) {
   const int side = ((int)(__float_as_uint(r) ^ u) >> 31) | 1;  // the exact quotient is larger (1) or smaller (-1)
   return r != 0.0f && (u & 1u) == 0u ? __uint_as_float(u + (uint32_t)side) : q;
 }
-// x / h, correctly rounded, from y = the rounded reciprocal of h (P. Markstein, IBM J. R&D 34(1), 1990),
-// while neither h, x nor the quotient is near the ends of fp32's range.
-__device__ __forceinline__ float quotient(float x, float h, float y) {
+// Such a quotient from y = the rounded reciprocal of h (P. Markstein, IBM J. R&D 34(1), 1990), with the
+// divisor's rest l in the correction: x / h alone, correctly rounded, can be a step and a half from x / (h + l), on
+// the other side of a border.  While neither h, x nor the quotient is near the ends of fp32's range.
+__device__ __forceinline__ float quotient(float x, float h, float l, float y) {
   const float q = x * y;
-  return fmaf(fmaf(-q, h, x), y, q);
+  return fmaf(fmaf(-q, l, fmaf(-q, h, x)), y, q);
 }
 
 // nvfp4 scale byte: e4m3(amax / (6 g)) of the exact quotient, through a quotient rounded to odd (in 64
@@ -96,7 +97,7 @@ __device__ __forceinline__ uint32_t nvfp4_scale_byte(uint32_t amax_bits, float g
   const float h = 6.0f * g, l = fmaf(6.0f, g, -h);
   float t;
   if (h >= 1.0e-25f && h <= 1.0e25f && amax <= h * 65536.0f) {
-    t = to_odd(quotient(amax, h, __frcp_rn(h)), amax, h, l);
+    t = to_odd(quotient(amax, h, l, __frcp_rn(h)), amax, h, l);
   } else {
     const double d = (double)amax / (6.0 * (double)g);
     if (!(amax_bits < 0x7F800000u && g > 0.0f && __float_as_uint(g) < 0x7F800000u)) return 0x7Fu;
@@ -202,13 +203,14 @@ __device__ __forceinline__ uint2 nvfp4_codes(const float (&x)[16], uint32_t amax
       q[i + 1] = f2_hi(p);
     }
   } else {
-    // Markstein's correction with -x: q0 = (-x)(-y), r = q0 d - x, q = q0 - r y, so that a zero keeps its sign
-    const uint64_t ny = f2_pack(-u.y, -u.y), dd = f2_pack(u.d, u.d);
+    // Markstein's correction with -x: q0 = (-x)(-y), r = q0 (d + dl) - x, q = q0 - r y, so that a zero keeps its sign
+    const float dl = fmaf(e4m3_value(byte), g, -u.d);
+    const uint64_t ny = f2_pack(-u.y, -u.y), dd = f2_pack(u.d, u.d), ll = f2_pack(dl, dl);
 #pragma unroll
     for (int i = 0; i < 16; i += 2) {
       const uint64_t xx = f2_pack(-x[i], -x[i + 1]);
       const uint64_t q0 = f2_mul(xx, ny);
-      const uint64_t p = f2_fma(f2_fma(q0, dd, xx), ny, q0);
+      const uint64_t p = f2_fma(f2_fma(q0, ll, f2_fma(q0, dd, xx)), ny, q0);
       q[i] = f2_lo(p);
       q[i + 1] = f2_hi(p);
     }
@@ -217,7 +219,6 @@ __device__ __forceinline__ uint2 nvfp4_codes(const float (&x)[16], uint32_t amax
 #pragma unroll
       for (int i = 0; i < 16; ++i) near_border |= (__float_as_uint(q[i]) & 0x1FFFFFu) == 0u;
       if (near_border) {
-        const float dl = fmaf(e4m3_value(byte), g, -u.d);
 #pragma unroll
         for (int i = 0; i < 16; ++i) q[i] = to_odd(q[i], x[i], u.d, dl);
       }
