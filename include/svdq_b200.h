@@ -489,7 +489,8 @@ int svdq_mx_dequantize(const void* codes, const void* scales, int format, const 
                        int M, int K, void* out, int64_t ldo, int dtype, cudaStream_t stream);
 
 /* *out = max |x| / (6 * 448), the nvfp4 tensor scale that puts the largest element on the largest
- * code and scale; 1 for a matrix of zeros, NaN where x has a NaN. */
+ * code and scale (rounded up where it is below fp32's normal range, so never 0); 1 for a matrix of zeros, NaN
+ * where x has a NaN. */
 int svdq_mx_tensor_scale(const void* x, int64_t ldx, int dtype, int M, int K, float* out, cudaStream_t stream);
 
 /*

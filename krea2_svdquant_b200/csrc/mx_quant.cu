@@ -257,10 +257,12 @@ __global__ void __launch_bounds__(kThreads) mx_amax_kernel(const T* x, int64_t l
   amax = __reduce_max_sync(0xffffffffu, amax);
   if ((threadIdx.x & 31) == 0) atomicMax(out, amax);
 }
-// amax bits -> the tensor scale amax / (6 * 448), 1 for a matrix of zeros.
+// amax bits -> the tensor scale amax / (6 * 448), 1 for a matrix of zeros.  Below fp32's normal range it is
+// rounded up: to nearest it can be 0, which is no scale, or so much too small that the largest elements saturate.
 __global__ void mx_tensor_scale_kernel(float* out) {
   const float amax = *out;
-  *out = amax == 0.0f ? 1.0f : amax / 2688.0f;
+  const float g = amax / 2688.0f;
+  *out = amax == 0.0f ? 1.0f : g < 0x1p-126f ? __fdiv_ru(amax, 2688.0f) : g;
 }
 
 // chunks and per_row of a matrix of `rows` rows in chunks of C columns; false where a launch cannot hold it
