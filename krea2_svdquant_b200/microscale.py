@@ -44,13 +44,15 @@ def _kernels():
 @dataclass(slots=True)
 class MicroTensor:
     """A block-scaled matrix: ``codes`` and ``scales`` as ``ops.mx_quantize`` writes them, the format,
-    the shape of the values (codes are the rows of ``shape`` flattened to 2-D) and nvfp4's tensor scale."""
+    the shape of the values (codes are the rows of ``shape`` flattened to 2-D), nvfp4's tensor scale and the
+    type of the values it was made from (None where that is not known), which a linear's output takes."""
 
     codes: torch.Tensor
     scales: torch.Tensor
     fmt: str
     shape: tuple[int, ...]
     tensor_scale: torch.Tensor | None = None
+    dtype: torch.dtype | None = None
 
     @property
     def device(self) -> torch.device:
@@ -79,7 +81,7 @@ def quantize(x: torch.Tensor, fmt: str = "nvfp4", *, tensor_scale: torch.Tensor 
     (None: 1); for weights use :func:`tensor_scale`.  Codes are those of the exact quotients, ties to
     even; a block with an infinity or a NaN reads back as NaN."""
     codes, scales = _kernels().mx_quantize(_rows(x), fmt, tensor_scale)
-    return MicroTensor(codes, scales, fmt, x.shape, tensor_scale)
+    return MicroTensor(codes, scales, fmt, x.shape, tensor_scale, x.dtype)
 
 
 def dequantize(t: MicroTensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
@@ -101,10 +103,11 @@ def matmul(a: MicroTensor, w: MicroTensor, bias: torch.Tensor | None = None, *,
 def linear(x: torch.Tensor | MicroTensor, w: MicroTensor, bias: torch.Tensor | None = None, *, act: str | None = None,
            act_scale: torch.Tensor | None = None, out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """``x @ w^T + bias`` with x quantised to format ``act`` on the way (None: the weight's own format;
-    ``act_scale``: its calibrated nvfp4 tensor scale).  The output has x's dtype unless ``out_dtype`` says otherwise.  An x that is
-    a :class:`MicroTensor` already goes straight to the product (bf16 output by default)."""
+    ``act_scale``: its calibrated nvfp4 tensor scale).  An x that is a :class:`MicroTensor` already goes
+    straight to the product.  The output has x's dtype (a MicroTensor's that of the values it was made from,
+    bf16 where that is not known) unless ``out_dtype`` says otherwise."""
     if isinstance(x, MicroTensor):
-        return matmul(x, w, bias, out_dtype=out_dtype or torch.bfloat16)
+        return matmul(x, w, bias, out_dtype=out_dtype or x.dtype or torch.bfloat16)
     if len(w.shape) != 2 or x.dim() < 1 or x.shape[-1] != w.shape[1]:
         raise ValueError(f"linear: activations {tuple(x.shape)} and weight {w.shape} do not match")
     out = _kernels().mx_linear(_rows(x), act or w.fmt, act_scale, w.codes, w.scales, w.fmt, w.tensor_scale, bias,
@@ -125,7 +128,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, *, residual: t
         total = x
     elif x.dim() != 2:
         total = total.reshape(x.shape)
-    return MicroTensor(codes, scales, "mxfp8", x.shape), total
+    return MicroTensor(codes, scales, "mxfp8", x.shape, None, x.dtype), total
 
 
 class MicroscaledLinear(nn.Module):
