@@ -172,11 +172,17 @@ class MicroscaledLinear(nn.Module):
         return cls(packed, None if layer.bias is None else layer.bias.detach(), act=act, act_scale=act_scale)
 
     def _apply(self, fn, recurse=True):
-        # .half() / .to(dtype) casts a model's floating buffers; these have one type each and only move
+        # .half() / .to(dtype) casts a model's floating buffers; these have one type each and only move, so
+        # they go through fn as integers
         kept = {n: b for n in ("weight_scale", "act_scale", "bias") if (b := self._buffers[n]) is not None}
-        super()._apply(fn, recurse)
-        for n, b in kept.items():
-            self._buffers[n] = b.to(self.codes.device)
+        views = {n: b.view(torch.int32 if b.element_size() == 4 else torch.int16) for n, b in kept.items()}
+        self._buffers.update(views)
+        try:
+            super()._apply(fn, recurse)
+        finally:
+            for n, b in kept.items():
+                t = self._buffers[n]
+                self._buffers[n] = b if t is views[n] else t.view(b.dtype)
         return self
 
     @property
