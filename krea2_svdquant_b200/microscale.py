@@ -135,7 +135,7 @@ class MicroscaledLinear(nn.Module):
     """A linear with a block-scaled 4-bit weight: ``act`` is the format of its activations (``nvfp4``,
     ``mxfp4``, or ``mxfp8`` for 8-bit activations on an mxfp4 weight).  ``forward`` takes a tensor, which
     it quantises, or a :class:`MicroTensor` in ``act``'s format (:func:`rms_norm`'s output), which
-    several layers can share.
+    several layers can share (with calibrated nvfp4 scales, layers that are given one ``act_scale`` tensor).
 
     ``check_device_errors``: as on :class:`~krea2_svdquant_b200.linear.SVDQuantLinear`."""
 

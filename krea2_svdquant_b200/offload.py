@@ -59,25 +59,25 @@ class _BlockArena:
             if id(p) not in seen:
                 seen.add(id(p))
                 params.append((p, p.data))
-        bufs: list[tuple[nn.Module, str, torch.Tensor]] = []
+        bufs: dict[int, tuple[torch.Tensor, list[tuple[nn.Module, str]]]] = {}  # a tensor and its owners
         for m in block.modules():
             for name, b in m._buffers.items():
                 if b is not None:
-                    bufs.append((m, name, b))
+                    bufs.setdefault(id(b), (b, []))[1].append((m, name))
         self._layout: list[tuple[int, int, torch.dtype, torch.Size]] = []
         off = 0
-        for t in [t for _, t in params] + [t for _, _, t in bufs]:
+        src = [t for _, t in params] + [t for t, _ in bufs.values()]
+        for t in src:
             nbytes = t.numel() * t.element_size()
             self._layout.append((off, nbytes, t.dtype, t.shape))
             off += (nbytes + _ALIGN - 1) // _ALIGN * _ALIGN
         self.nbytes = off
         self.host = torch.empty(max(off, 1), dtype=torch.uint8, pin_memory=pin)
         views = self._views(self.host)
-        src = [t for _, t in params] + [t for _, _, t in bufs]
         for v, t in zip(views, src):
             v.copy_(t.contiguous())
         self._params = params
-        self._bufs = bufs
+        self._bufs = [owners for _, owners in bufs.values()]
         self._cpu_views = views
         self._attach(views)
 
@@ -91,8 +91,9 @@ class _BlockArena:
         n = len(self._params)
         for (p, _), v in zip(self._params, views[:n]):
             p.data = v
-        for (m, name, _), v in zip(self._bufs, views[n:]):
-            m._buffers[name] = v
+        for owners, v in zip(self._bufs, views[n:]):
+            for m, name in owners:
+                m._buffers[name] = v
 
     def attach_device(self, base: torch.Tensor) -> None:
         self._attach(self._views(base))

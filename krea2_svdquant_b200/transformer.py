@@ -177,7 +177,8 @@ def _quantized_norm(norm: nn.RMSNorm, x: torch.Tensor, act: str, act_scale: torc
 
 
 def _shared_format(layers) -> tuple[str, torch.Tensor | None] | None:
-    """The activation format (and tensor scale) that block-scaled layers have in common, or None."""
+    """The activation format and tensor scale (one tensor, so that equal values need no look at the
+    device) that block-scaled layers have in common, or None."""
     layers = list(layers)
     if not all(isinstance(lin, MicroscaledLinear) for lin in layers):
         return None
@@ -192,6 +193,18 @@ class Krea2StandInBlock(nn.Module):
         self.attn = _Attention(cfg, lin)
         self.norm2 = nn.RMSNorm(cfg.hidden, eps=1e-6, dtype=dtype)
         self.ff = _FeedForward(lin)
+
+    def _apply(self, fn, recurse=True):
+        # layers with one act_scale tensor read one quantised input; a move gives each layer a copy of its own
+        shared: dict[int, list[MicroscaledLinear]] = {}
+        for lin in self.modules():
+            if isinstance(lin, MicroscaledLinear) and lin.act_scale is not None:
+                shared.setdefault(id(lin.act_scale), []).append(lin)
+        super()._apply(fn, recurse)
+        for first, *others in shared.values():
+            for lin in others:
+                lin.act_scale = first.act_scale
+        return self
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         # x + attn(norm1(x)), then x + ff(norm2(x)); the residual adds (and the gate products
