@@ -169,11 +169,19 @@ def _linear(lin: nn.Module, x: torch.Tensor, epilogue: tuple[str, torch.Tensor] 
 def _quantized_norm(norm: nn.RMSNorm, x: torch.Tensor, act: str, act_scale: torch.Tensor | None,
                     residual: torch.Tensor | None = None) -> tuple[MicroTensor, torch.Tensor]:
     """``(norm(h) in format act, h)`` with ``h = x + residual``: the input of several block-scaled
-    linears, quantised once.  For mxfp8 the add, the norm and the quantisation are one kernel."""
-    if act == "mxfp8":
+    linears, quantised once.  For mxfp8 the add, the norm and the quantisation are one kernel, where the
+    norm is a plain one (a subclass, hooks, no epsilon of its own or a weight in another type: the module runs)."""
+    if act == "mxfp8" and _plain_norm(norm, x):
         return microscale.rms_norm(x, norm.weight, residual=residual, eps=norm.eps)
     h = x if residual is None else x + residual
     return microscale.quantize(norm(h), act, tensor_scale=act_scale), h
+
+
+def _plain_norm(norm: nn.Module, x: torch.Tensor) -> bool:
+    hooks = (norm._forward_hooks, norm._forward_pre_hooks, nn.modules.module._global_forward_hooks,
+             nn.modules.module._global_forward_pre_hooks)
+    return (type(norm) is nn.RMSNorm and not any(hooks) and "forward" not in norm.__dict__ and norm.eps is not None
+            and (norm.weight is None or norm.weight.dtype == x.dtype) and norm.normalized_shape == x.shape[-1:])
 
 
 def _shared_format(layers) -> tuple[str, torch.Tensor | None] | None:
