@@ -496,7 +496,8 @@ int svdq_mx_tensor_scale(const void* x, int64_t ldx, int dtype, int M, int K, fl
 /*
  * Block-scaled GEMM: out[m, n] = g_a g_w sum_k A[m, k] W[n, k] + bias[n], on the tensor cores'
  * block-scaled MMAs with fp32 accumulation.  Formats (activations x weight): nvfp4 x nvfp4,
- * mxfp4 x mxfp4, mxfp8 x mxfp4.  Tensor scales: one fp32 device value each (nvfp4 only; NULL for 1).
+ * mxfp4 x mxfp4, mxfp8 x mxfp4.  Tensor scales: one fp32 device value each (nvfp4 only; NULL for 1), whose
+ * product is formed in fp32.
  * bias [N] bf16 or NULL.  out [M, N] in out_dtype, row stride ldo >= N, any N.  The sums are added in
  * a fixed order: the same call gives the same bits.
  *   codes and scales 32-byte aligned; M, N <= 2^24, K <= 2^28.

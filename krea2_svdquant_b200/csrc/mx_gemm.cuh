@@ -115,8 +115,16 @@ struct MxInput {
   int dtype;
   bool vec;  // rows on 32-byte boundaries and K a multiple of 16
 };
-// Up to 4 tokens: 128 columns or more of each, a warp's work or two per stage.  N 16384, K 6144, nvfp4:
-// 13.4 us against 15.4 with a quantisation before at 4 tokens, 15.7 against 15.4 at 5.
+// Up to 4 tokens: 128 columns or more of each, a warp's work or two per stage.  Each CTA quantises its share of
+// K again, so more tokens cost more the more tiles of weight rows there are.  us against a quantisation before
+// (weight out of L2):
+//                              4 tokens       5              8
+//   nvfp4  bf16  N 16384 K 6144  12.8 / 14.9   15.4 / 15.1   18.4 / 15.5
+//   nvfp4  bf16  N 1536  K 6144   5.5 / 7.0     6.6 / 6.9     6.7 / 7.0
+//   mxfp8  bf16  N 16384 K 6144  13.5 / 15.4   16.4 / 15.3   17.1 / 15.9
+//   mxfp4  fp32  N 6144  K 16384 13.6 / 14.4   15.8 / 14.4   18.5 / 14.5
+// From fp32 to nvfp4, whose units cost most, 3 and 4 tokens are up to 11% slower at N 16384 or K 16384 (17.4 / 15.8)
+// and 8% faster at N 1536; they keep the limit of the others, as the workspace's size does not know the type.
 constexpr int kMaxFusedTokens = 4;
 
 // One checked GEMM call.

@@ -457,7 +457,9 @@ int launch_split(const MxGemm& g, const SplitPlan& p) {
 
 // One product: the pair kernel or this one, whichever is estimated to end first.  A tile of the pair
 // kernel costs 0.42 (nvfp4), 0.40 (mxfp4) or 0.36 us (mxfp8 x mxfp4) per stage.  At N 6144, K 6144,
-// mxfp8 on mxfp4: 128 tokens 16.2 us here against 21.2 on pairs, 256 tokens 25.8 against 21.4.
+// mxfp8 on mxfp4: 128 tokens 16.2 us here against 21.2 on pairs, 256 tokens 25.8 against 21.4.  Both timed for 204 calls
+// (8 to 4352 tokens, four weights, three modes, weight out of L2), the estimate's choice was slower by more than 1%
+// in one, by 3%.
 template <int MODE, int TN>
 int choose(const MxGemm& g) {
   constexpr float kPairUs[3] = {.42f, .40f, .36f};
@@ -485,12 +487,6 @@ int choose_tokens(const MxGemm& g) {
   if (g.o.M <= 64) return choose<MODE, 64>(g);
   return choose<MODE, 128>(g);
 }
-
-}  // namespace
-}  // namespace svdq
-
-namespace svdq {
-namespace {
 
 // Checks a product's arguments (the activations as codes and scales, or g.in) and runs it.
 int mx_product(MxGemm& g, int K) {
