@@ -34,6 +34,7 @@ from torch import nn
 from . import _lib, ops
 
 FORMATS = tuple(ops.MX_BLOCK)
+_INTEGER = {2: torch.int16, 4: torch.int32, 8: torch.int64}  # by bytes
 ACTIVATIONS = {act: w for act, w in ops.MX_PRODUCTS}  # activation format -> the weight format it multiplies
 
 
@@ -175,7 +176,7 @@ class MicroscaledLinear(nn.Module):
         # .half() / .to(dtype) casts a model's floating buffers; these have one type each and only move, so
         # they go through fn as integers
         kept = {n: b for n in ("weight_scale", "act_scale", "bias") if (b := self._buffers[n]) is not None}
-        views = {n: b.view(torch.int32 if b.element_size() == 4 else torch.int16) for n, b in kept.items()}
+        views = {n: b.view(_INTEGER[b.element_size()]) for n, b in kept.items()}
         self._buffers.update(views)
         try:
             super()._apply(fn, recurse)

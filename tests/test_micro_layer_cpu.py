@@ -47,3 +47,9 @@ def test_a_move_that_moves_nothing_keeps_the_tensors():
 def test_shared_memory():
     lin = layer(torch.tensor([0.7])).share_memory()
     assert all(b.is_shared() for b in lin.buffers())
+
+
+def test_a_scale_in_another_type_moves_too():
+    """Refused where it is used, not where it is moved."""
+    lin = layer(torch.tensor([0.7], dtype=torch.float64)).to("meta").to_empty(device="cpu")
+    assert lin.act_scale.dtype == torch.float64 and lin.act_scale.device.type == "cpu"
