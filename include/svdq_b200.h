@@ -523,8 +523,8 @@ int svdq_mx_linear(const void* x, int64_t ldx, int dtype, int a_format, const fl
 /*
  * Root-mean-square norm with the residual's addition, written as mxfp8:
  *   h = x + residual (rounded to dtype; stored to sum),  y = h * rsqrt(mean(h^2) + eps) * weight,
- *   y quantised to SVDQ_MX_MXFP8: codes and scales are those of the exact y (taken for a value between two
- *   codes when within 2^-46 of it), for h and weight of any finite size.  A y past fp32's range is an infinity.
+ *   y quantised to SVDQ_MX_MXFP8: codes and scales are those of the exact y (taken to lie on a border between two
+ *   codes or scales when within 2^-46 of it), for h and weight of any finite size.  A y past fp32's range is an infinity.
  * x, residual, sum [M, H] and weight [H] in dtype (bf16, fp16, fp32), row strides ldx, ldr, lds;
  * residual and sum both NULL: h = x.  weight NULL: ones.  sum may be x or residual itself (with the
  * same stride).  codes [M, round_up(H, 128)] and scales as svdq_mx_quantize writes them.

@@ -87,6 +87,7 @@ __device__ __forceinline__ void encode_exactly(const NormArgs& a, int row, const
   alignas(32) T h[C], w[C];
   load_columns<VEC>(h_row, c, a.H, h);
   if (a.weight) load_columns<VEC>(static_cast<const T*>(a.weight), c, a.H, w);
+  if (c >= a.H) root = 0.0;  // a row's root can be infinite or NaN, the blocks that pad it hold zeros all the same
   float y[C];
 #pragma unroll
   for (int i = 0; i < C; ++i) {

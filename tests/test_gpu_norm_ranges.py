@@ -82,3 +82,22 @@ def test_ranges_meet_in_one_matrix():
     y[:, 64:128] = 0  # whole blocks of zeros
     check(y, None, 1e-6)
 
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("h", [1, 40, 300, 1111, 20001])
+def test_padding_of_rows_without_a_norm(dtype, h):
+    """Zeros without eps (0 / 0), an infinity, a NaN: the row's own blocks are NaN where the norm is, those that fill it
+    up to 128 columns hold zeros."""
+    from krea2_svdquant_b200 import microscale as M
+    x = torch.ones(5, h, device="cuda", dtype=dtype)
+    x[0] = 0
+    x[1, h // 2] = float("nan")
+    x[2, h // 2] = float("inf")
+    for w in (None, torch.ones(h, device="cuda", dtype=dtype)):
+        q, _ = M.rms_norm(x, w, eps=0.0)
+        byte = torch.from_numpy(q.scales.cpu().numpy()[O.scale_index(5, O.k_pad(h) // 32)])
+        own = -(-h // 32)
+        assert (byte[:2, :own] == 255).all() and (byte[:, own:] == 0).all()
+        assert byte[2, h // 64] == 255 and (byte[2, :own] == 255).sum() == 1
+        assert (byte[3:, :own] == 119).all()  # 2^-8: a norm of ones
+        assert not q.codes.view(torch.uint8)[:, h:].any()
