@@ -120,7 +120,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, *, residual: t
              eps: float = 1e-6) -> tuple[MicroTensor, torch.Tensor]:
     """``(norm, h)``: ``h = x + residual`` in x's dtype (x itself without a residual) and the
     root-mean-square norm ``h * rsqrt(mean(h^2) + eps) * weight`` over the last dimension as mxfp8, with
-    the codes and scales of its exact value."""
+    the codes and scales of its exact value (``eps`` as fp32)."""
     x2 = _rows(x)
     if residual is not None and residual.shape != x.shape:
         raise ValueError(f"rms_norm: residual {tuple(residual.shape)} must have x's shape {tuple(x.shape)}")
